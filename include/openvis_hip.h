@@ -22,6 +22,11 @@ extern "C" {
 #define OVIS_EINVAL 1   /* bad argument (null pointer, non-positive size, unsupported shape) */
 #define OVIS_ELAUNCH 2  /* hipLaunchKernel / runtime error */
 
+/* Element types of the training-side operators (layer norm, relative position bias, 8-bit activations, weight gradient). */
+#define OVIS_F32 0
+#define OVIS_F16 1
+#define OVIS_BF16 2
+
 typedef void* ovis_stream_t; /* hipStream_t */
 
 /* Library ABI version (bumped when a signature changes). */
@@ -549,6 +554,29 @@ int ovis_pil_resize_u8_hwc_to_chw(const uint8_t* src, int H, int W, uint8_t* tmp
 int ovis_pil_resize_preprocess_u8(const uint8_t* src, int H, int W, uint8_t* tmp, uint8_t* dst, float* img_nhwc4, int OH, int OW, int Hp,
                                   int Wp, const int* xbounds, const int* xk, int xksize, const int* ybounds, const int* yk, int yksize,
                                   const float* mean3_host, const float* std3_host, ovis_stream_t stream);
+
+/* ==== Training-side operators ==================================================================================
+ * What a fine-tuning step of the transformer blocks on the path needs next to their forward kernels.  Types are OVIS_F32 / OVIS_F16 /
+ * OVIS_BF16; arithmetic, sums and statistics are f32; rows are `ld` elements apart with contiguous elements, no alignment needed.
+ *
+ * 8-bit form of a matrix [rows, C]: e4m3 codes u8 [rows, C] and one scale u8 (e8m0: 2^(byte - 127)) [rows, ceil(C / 32)] per 32 columns --
+ * the smallest power of two in [2^-100, 2^120] under which the largest finite magnitude of the 32 is at most 448.  NaN and infinities are
+ * NaN codes. */
+
+/* Layer norm with what its backward pass needs (the reference trains nn.LayerNorm, e.g. msdeformattn.py:139-146, swin.py:224-284).
+ *   forward: s = x + residual rounded to x's type (written to sum [rows, C]; residual and sum NULL: s = x); y = (s - mean) rstd gamma + beta;
+ *     stats f32 [rows, 2] = (mean, rstd); codes / scales (both or neither NULL): (s - mean) rstd in 8 bits.
+ *     y_dtype = x_dtype, or any where x is f32; C <= 8192.
+ *   backward: dx = rstd (dy gamma - mean(dy gamma) - xhat mean(dy gamma xhat)) + dsum (NULL: none), dgamma = sum dy xhat, dbeta = sum dy
+ *     (fixed order: the same bits at every call); xhat from x [rows, ldx] and stats, or from codes / scales (x NULL; the mean is not used).
+ *     dx and dsum have x_dtype; workspace of ovis_layernorm_train_backward_workspace_bytes(rows, C) bytes. */
+int ovis_layernorm_train_forward(const void* x, long long ldx, const void* residual, long long ldr, const float* gamma, const float* beta,
+                                 void* sum, void* y, float* stats, uint8_t* codes, uint8_t* scales, long long rows, int C, float eps,
+                                 int x_dtype, int y_dtype, ovis_stream_t stream);
+long long ovis_layernorm_train_backward_workspace_bytes(long long rows, int C);
+int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x, long long ldx, const uint8_t* codes, const uint8_t* scales,
+                                  const float* stats, const float* gamma, const void* dsum, long long ldds, void* dx, float* dgamma,
+                                  float* dbeta, float* workspace, long long rows, int C, int dy_dtype, int x_dtype, ovis_stream_t stream);
 
 #ifdef __cplusplus
 }

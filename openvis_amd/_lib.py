@@ -40,7 +40,8 @@ def lib():
         _lib.ovis_last_error.restype = ctypes.c_char_p
         _lib.ovis_abi_version.restype = ctypes.c_int
         for fn in ("ovis_attention_workspace_bytes", "ovis_hungarian_link_workspace_bytes", "ovis_clip_crop_workspace_bytes",
-                   "ovis_attention_partial_floats", "ovis_attention_partial_workspace_bytes"):
+                   "ovis_attention_partial_floats", "ovis_attention_partial_workspace_bytes",
+                   "ovis_layernorm_train_backward_workspace_bytes"):
             if hasattr(_lib, fn):
                 getattr(_lib, fn).restype = ctypes.c_longlong
     return _lib
@@ -76,8 +77,10 @@ def _throttle():
     if n < LAUNCH_WINDOW:
         _tls.n = n
         return
-    _tls.n = 0
     import torch
+    if torch.cuda.is_current_stream_capturing():      # an event recorded into a graph cannot be waited for: count on after the capture
+        return
+    _tls.n = 0
     ev = torch.cuda.Event()
     ev.record()
     q = getattr(_tls, "q", None)

@@ -1,0 +1,312 @@
+// Layer norm for training on gfx950: forward with the row statistics and, if asked, the normalised rows in 8 bits; backward with the input,
+// weight and bias gradients.
+//
+//   s    = x + residual, rounded to x's type (what the next layer and the backward pass see)
+//   xhat = (s - mean) * rstd,  y = xhat * gamma + beta           mean, rstd = 1/sqrt(var + eps): two passes over registers, f32
+//   gd   = dy * gamma
+//   dx   = rstd * (gd - mean(gd) - xhat * mean(gd * xhat)) + dsum
+//   dgamma = sum over rows dy * xhat,  dbeta = sum over rows dy
+//
+// Bound by HBM: every input is read once and every output written once.  LPR neighbouring lanes hold a row in registers, 8 columns a lane and
+// NCH such pieces each (256 lanes = a whole workgroup from 2049 columns on), so a row is read once although forward needs it three times.
+// The weight gradient is summed over rows in a fixed order: a workgroup keeps the sums of its rows in registers, writes one line of the
+// workspace, and a second kernel adds the lines (no atomics: the same bits at every call).
+#include "train_elem.h"
+
+namespace {
+
+using namespace ovis;
+
+// sum over the LPR lanes of a row; LPR = 256 crosses the four wavefronts through `buf` (two alternating slots, so that one barrier is enough)
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* buf) {
+#pragma unroll
+  for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (LPR > 64) {
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+  }
+  return v;
+}
+
+template <typename TX, typename TY, int LPR, int NCH>
+__global__ void __launch_bounds__(256)
+layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __restrict__ res, long long ldr, const float* __restrict__ gamma,
+                           const float* __restrict__ beta, TX* __restrict__ sum, TY* __restrict__ y, float* __restrict__ stats,
+                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, long long rows, int C, float eps) {
+  __shared__ float buf[2][4];
+  const int li = threadIdx.x % LPR;
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const bool live = row < rows;                                  // lanes of a row behind the last one stay for the shuffles
+  const long long r = live ? row : rows - 1;
+  float v[NCH][8];
+  float s = 0.f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * LPR + li) * 8, n = C - col;
+    if (n > 0) {
+      load8(x + r * ldx + col, n, v[c]);
+      if (res) {
+        float t[8];
+        load8(res + r * ldr + col, n, t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[c][e] = (float)(TX)(v[c][e] + t[e]);
+        if (live) store8(sum + r * C + col, n, v[c]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[c][e];
+  }
+  const float mean = row_sum<LPR>(s, buf[0]) / (float)C;
+  float q = 0.f;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int n = C - (c * LPR + li) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[c][e] = e < n ? v[c][e] - mean : 0.f;
+      q += v[c][e] * v[c][e];
+    }
+  }
+  const float rstd = 1.f / sqrtf(row_sum<LPR>(q, buf[1]) / (float)C + eps);
+  if (live && li == 0) {
+    stats[2 * r] = mean;
+    stats[2 * r + 1] = rstd;
+  }
+  const int nblk = (C + 31) >> 5;
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * LPR + li) * 8, n = C - col;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[c][e] *= rstd;
+    if (codes) {                                                 // all four lanes of a block take part, the ones behind the row's end with 0
+      unsigned sb;
+      const u32x2_u q8 = encode8(v[c], false, sb);
+      if (live && n > 0) {
+        store_codes(codes + r * C + col, n, q8);
+        if ((li & 3) == 0) scales[r * nblk + (col >> 5)] = (uint8_t)sb;
+      }
+    }
+    if (live && n > 0) {
+      float g[8], b[8];
+      load8(gamma + col, n, g);
+      load8(beta + col, n, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[c][e] = v[c][e] * g[e] + b[e];
+      store8(y + r * C + col, n, v[c]);
+    }
+  }
+}
+
+// TX: x, dsum and dx; TY: dy.  A workgroup walks over rows and keeps dgamma / dbeta of its lanes' columns in registers.
+template <typename TX, typename TY, int LPR, int NCH>
+__global__ void __launch_bounds__(256)
+layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
+                           const uint8_t* __restrict__ scales, const float* __restrict__ stats, const float* __restrict__ gamma,
+                           const TX* __restrict__ dsum, long long ldds, TX* __restrict__ dx, float* __restrict__ part, long long rows, int C) {
+  __shared__ float buf[4][4];
+  extern __shared__ float acc[];                                 // [2][C]: the workgroup's sums
+  const int li = threadIdx.x % LPR;
+  constexpr int RPB = 256 / LPR;
+  const int nblk = (C + 31) >> 5;
+  float g[NCH][8], dg[NCH][8], db[NCH][8];
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int col = (c * LPR + li) * 8, n = C - col;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[c][e] = dg[c][e] = db[c][e] = 0.f;
+    if (n > 0) load8(gamma + col, n, g[c]);
+  }
+  int phase = 0;
+  for (long long r0 = (long long)blockIdx.x * RPB; r0 < rows; r0 += (long long)gridDim.x * RPB) {
+    const long long row = r0 + threadIdx.x / LPR;
+    const bool live = row < rows;
+    const long long r = live ? row : rows - 1;
+    const float mean = stats[2 * r], rstd = stats[2 * r + 1];
+    float d[NCH][8], h[NCH][8];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * LPR + li) * 8, n = C - col;
+      if (n > 0 && live) {
+        load8(dy + r * lddy + col, n, d[c]);
+        if (codes) {
+          decode8(load_codes(codes + r * C + col, n), scales[r * nblk + (col >> 5)], h[c]);
+        } else {
+          load8(x + r * ldx + col, n, h[c]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[c][e] = e < n ? (h[c][e] - mean) * rstd : 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[c][e] = h[c][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float gd = d[c][e] * g[c][e];
+        s1 += gd;
+        s2 += gd * h[c][e];
+        dg[c][e] += d[c][e] * h[c][e];
+        db[c][e] += d[c][e];
+      }
+    }
+    const float c1 = row_sum<LPR>(s1, buf[2 * phase]) / (float)C;
+    const float c2 = row_sum<LPR>(s2, buf[2 * phase + 1]) / (float)C;
+    phase ^= 1;
+#pragma unroll
+    for (int c = 0; c < NCH; ++c) {
+      const int col = (c * LPR + li) * 8, n = C - col;
+      if (n > 0 && live) {
+        float o[8], t[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = rstd * (d[c][e] * g[c][e] - c1 - h[c][e] * c2);
+        if (dsum) {
+          load8(dsum + r * ldds + col, n, t);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] += t[e];
+        }
+        store8(dx + r * C + col, n, o);
+      }
+    }
+  }
+  // the rows of a workgroup, in order: lanes of the same columns are LPR apart
+  for (int k = 0; k < RPB; ++k) {
+    if ((int)threadIdx.x / LPR == k) {
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int col = (c * LPR + li) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (col + e < C) {
+            acc[col + e] = (k ? acc[col + e] : 0.f) + dg[c][e];
+            acc[C + col + e] = (k ? acc[C + col + e] : 0.f) + db[c][e];
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float* line = part + (long long)blockIdx.x * 2 * C;
+  for (int i = threadIdx.x; i < 2 * C; i += 256) line[i] = acc[i];
+}
+
+struct RowShape { int lpr, nch; };
+// Lanes per row: the fewest that hold the row in four pieces each, since a lane's extra pieces are loads in flight while a lane behind the
+// row's end is idle.
+inline RowShape row_shape(int C) {
+  const int nvec = (C + 7) / 8;
+  for (int lpr : {16, 32, 64, 256})
+    if ((nvec + lpr - 1) / lpr <= 4) return {lpr, (nvec + lpr - 1) / lpr};
+  return {0, 0};
+}
+
+inline unsigned bwd_blocks(long long rows, int C) {
+  const RowShape s = row_shape(C);
+  const long long need = (rows + 256 / s.lpr - 1) / (256 / s.lpr);
+  return (unsigned)(need < 1024 ? need : 1024);
+}
+
+}  // namespace
+
+namespace ovis {
+
+// out0[w] (w < split), out1[w - split] = sum over the P lines of part [P][W], in a fixed order: 64 lanes of a column take every 64th line,
+// then a tree.  16 columns a workgroup: enough workgroups that the lines, which come from L2, are read in a few microseconds.
+__global__ void __launch_bounds__(1024)
+column_sum_finish_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
+  __shared__ float buf[64][17];
+  const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4;
+  const int w = blockIdx.x * 16 + c;
+  float s = 0.f;
+  if (w < W)
+    for (int p = p0; p < P; p += 64) s += part[(long long)p * W + w];
+  buf[p0][c] = s;
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (p0 < o) buf[p0][c] += buf[p0 + o][c];
+    __syncthreads();
+  }
+  if (p0 == 0 && w < W) {
+    if (w < split) out0[w] = buf[0][c];
+    else out1[w - split] = buf[0][c];
+  }
+}
+
+int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream) {
+  hipLaunchKernelGGL(column_sum_finish_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, part, P, W, out0, split, out1);
+  return check_launch("column_sum_finish");
+}
+
+}  // namespace ovis
+
+#define LN_TYPES(xt, yt, CALL)                                                                      \
+  if (xt == OVIS_F32 && yt == OVIS_F32) { CALL(float, float) }                                      \
+  else if (xt == OVIS_F32 && yt == OVIS_F16) { CALL(float, _Float16) }                              \
+  else if (xt == OVIS_F32) { CALL(float, __bf16) }                                                  \
+  else if (xt == OVIS_F16) { CALL(_Float16, _Float16) }                                             \
+  else { CALL(__bf16, __bf16) }
+#define LN_SHAPES(sh, TX, TY)                                                                       \
+  switch (sh.lpr * 8 + sh.nch) {                                                                    \
+    case 16 * 8 + 1: LN_GO(TX, TY, 16, 1); break;                                                   \
+    case 16 * 8 + 2: LN_GO(TX, TY, 16, 2); break;                                                   \
+    case 16 * 8 + 3: LN_GO(TX, TY, 16, 3); break;                                                   \
+    case 16 * 8 + 4: LN_GO(TX, TY, 16, 4); break;                                                   \
+    case 32 * 8 + 3: LN_GO(TX, TY, 32, 3); break;                                                   \
+    case 32 * 8 + 4: LN_GO(TX, TY, 32, 4); break;                                                   \
+    case 64 * 8 + 3: LN_GO(TX, TY, 64, 3); break;                                                   \
+    case 64 * 8 + 4: LN_GO(TX, TY, 64, 4); break;                                                   \
+    case 256 * 8 + 2: LN_GO(TX, TY, 256, 2); break;                                                 \
+    case 256 * 8 + 3: LN_GO(TX, TY, 256, 3); break;                                                 \
+    default: LN_GO(TX, TY, 256, 4); break;                                                          \
+  }
+
+extern "C" int ovis_layernorm_train_forward(const void* x, long long ldx, const void* residual, long long ldr, const float* gamma,
+                                            const float* beta, void* sum, void* y, float* stats, uint8_t* codes, uint8_t* scales,
+                                            long long rows, int C, float eps, int x_dtype, int y_dtype, ovis_stream_t stream) {
+  OVIS_REQUIRE(x && gamma && beta && y && stats && (!residual || sum) && (!codes == !scales), "layernorm_train_forward: null pointer");
+  OVIS_REQUIRE(rows > 0 && C > 0 && C <= 8192, "layernorm_train_forward: rows %lld, columns %d (1 to 8192)", rows, C);
+  OVIS_REQUIRE(ldx >= C && (!residual || ldr >= C), "layernorm_train_forward: row stride below the row length");
+  OVIS_REQUIRE(ovis::dtype_ok(x_dtype) && ovis::dtype_ok(y_dtype) && (x_dtype == OVIS_F32 || x_dtype == y_dtype),
+               "layernorm_train_forward: y has x's type, or any where x is f32");
+  const RowShape sh = row_shape(C);
+  const long long blocks = (rows + 256 / sh.lpr - 1) / (256 / sh.lpr);
+  OVIS_REQUIRE(blocks < (1ll << 31), "layernorm_train_forward: %lld rows are too many for one launch", rows);
+#define LN_GO(TX, TY, LPR, NCH)                                                                                                             \
+  hipLaunchKernelGGL((layernorm_train_fwd_kernel<TX, TY, LPR, NCH>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,            \
+                     (const TX*)x, ldx, (const TX*)residual, ldr, gamma, beta, (TX*)sum, (TY*)y, stats, codes, scales, rows, C, eps)
+#define LN_ALL(TX, TY) LN_SHAPES(sh, TX, TY)
+  LN_TYPES(x_dtype, y_dtype, LN_ALL)
+#undef LN_GO
+  return ovis::check_launch("layernorm_train_forward");
+}
+
+extern "C" long long ovis_layernorm_train_backward_workspace_bytes(long long rows, int C) {
+  if (rows <= 0 || C <= 0 || C > 8192) return 0;
+  return (long long)bwd_blocks(rows, C) * 2 * C * 4;
+}
+
+extern "C" int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x, long long ldx, const uint8_t* codes,
+                                             const uint8_t* scales, const float* stats, const float* gamma, const void* dsum, long long ldds,
+                                             void* dx, float* dgamma, float* dbeta, float* workspace, long long rows, int C, int dy_dtype,
+                                             int x_dtype, ovis_stream_t stream) {
+  OVIS_REQUIRE(dy && stats && gamma && dx && dgamma && dbeta && workspace && (!codes == !scales) && (!x != !codes),
+               "layernorm_train_backward: null pointer, or not exactly one of x and codes");
+  OVIS_REQUIRE(rows > 0 && C > 0 && C <= 8192, "layernorm_train_backward: rows %lld, columns %d (1 to 8192)", rows, C);
+  OVIS_REQUIRE(lddy >= C && (!x || ldx >= C) && (!dsum || ldds >= C), "layernorm_train_backward: row stride below the row length");
+  OVIS_REQUIRE(ovis::dtype_ok(dy_dtype) && ovis::dtype_ok(x_dtype) && (x_dtype == OVIS_F32 || x_dtype == dy_dtype),
+               "layernorm_train_backward: dy has x's type, or any where x is f32");
+  const RowShape sh = row_shape(C);
+  const unsigned blocks = bwd_blocks(rows, C);
+#define LN_GO(TX, TY, LPR, NCH)                                                                                                             \
+  hipLaunchKernelGGL((layernorm_train_bwd_kernel<TX, TY, LPR, NCH>), dim3(blocks), dim3(256), 2 * C * 4, (hipStream_t)stream,              \
+                     (const TY*)dy, lddy, (const TX*)x, ldx, codes, scales, stats, gamma, (const TX*)dsum, ldds, (TX*)dx, workspace, rows, C)
+  LN_TYPES(x_dtype, dy_dtype, LN_ALL)
+#undef LN_GO
+  const int rc = ovis::check_launch("layernorm_train_backward");
+  if (rc != OVIS_OK) return rc;
+  return ovis::column_sum_finish(workspace, (int)blocks, 2 * C, dgamma, C, dbeta, (hipStream_t)stream);
+}

@@ -1,0 +1,140 @@
+// Element types, unaligned 8-element vectors and the 8-bit block format of the training-side operators (gfx950 only).
+//
+// Types: OVIS_F32 / OVIS_F16 / OVIS_BF16 tensors; all arithmetic is f32 and each output is rounded once (to nearest even).
+// A lane moves 8 consecutive elements; rows need no alignment beyond the element's own (the hardware takes 16-byte global accesses at any
+// address), so odd row lengths and strided views use the same vector accesses as aligned ones and only a row's last lane goes by elements.
+//
+// 8-bit block format: e4m3 codes and one power-of-two scale (e8m0: 2^(byte - 127)) per 32 columns of a row.  Four neighbouring lanes hold a
+// block.  The scale is the smallest power of two in [2^-100, 2^120] under which the block's largest finite magnitude is at most 448, so no
+// value saturates and every value above 2^-6 of its scale is off by at most 2^-4 of itself.  The limits keep scale, value and their product
+// inside f32's normal range.  e4m3 has no infinity: infinities and NaN become the NaN code and do not take part in the block's maximum.
+#pragma once
+#include "common.h"
+
+namespace ovis {
+
+template <typename T> struct Vec8Of;                     // 8 elements, aligned as one element
+typedef _Float16 f16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 bf16x8_u __attribute__((ext_vector_type(8), aligned(2)));
+typedef float f32x8_u __attribute__((ext_vector_type(8), aligned(4)));
+template <> struct Vec8Of<_Float16> { using type = f16x8_u; };
+template <> struct Vec8Of<__bf16> { using type = bf16x8_u; };
+template <> struct Vec8Of<float> { using type = f32x8_u; };
+typedef unsigned u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
+
+// n (1..8) elements of p into v, the others 0
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)[8]) {
+  if (n >= 8) {
+    const typename Vec8Of<T>::type t = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v)[8]) {
+  if (n >= 8) {
+    typename Vec8Of<T>::type t;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+    *reinterpret_cast<typename Vec8Of<T>::type*>(p) = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (T)v[e];
+  }
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }   // -126 <= e <= 127
+
+// maximum over the four lanes of a block (quad_perm moves inside groups of four lanes: no LDS)
+__device__ __forceinline__ float quad_max(float a) {
+  int t = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, a), 0xB1, 0xf, 0xf, true);      // lanes 1 0 3 2
+  a = fmaxf(a, __builtin_bit_cast(float, t));
+  t = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, a), 0x4E, 0xf, 0xf, true);          // lanes 2 3 0 1
+  return fmaxf(a, __builtin_bit_cast(float, t));
+}
+
+// 8 values of one lane (the block's other 24 in its three neighbours; all four lanes active) -> 8 codes, and the scale's byte.
+// signed_zero: a value of 0 gets the code -0, so that a code's sign bit says "not positive" (ReLU's derivative).
+__device__ __forceinline__ u32x2_u encode8(const float (&v)[8], bool signed_zero, unsigned& scale_byte) {
+  float a = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));          // fmaxf passes a NaN over
+  a = quad_max(a);
+  float w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = v[e];
+  if (a == INFINITY) {                                             // rare: the maximum of the finite ones, infinities to NaN
+    a = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool inf = fabsf(w[e]) == INFINITY;
+      a = fmaxf(a, inf ? 0.f : fabsf(w[e]));
+      w[e] = inf ? NAN : w[e];
+    }
+    a = quad_max(a);
+  }
+  const unsigned bits = __builtin_bit_cast(unsigned, a);
+  int s = (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);       // 1.75 * 2^8 = 448
+  s = min(max(s, -100), 120);
+  scale_byte = (unsigned)(s + 127);
+  const float f = pow2f(-s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = signed_zero && w[e] == 0.f ? -0.f : w[e] * f;
+  u32x2_u r;
+  int t = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], 0, false);
+  t = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], t, true);
+  r[0] = (unsigned)t;
+  t = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], 0, false);
+  t = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], t, true);
+  r[1] = (unsigned)t;
+  return r;
+}
+
+// 8 codes -> the values they stand for (exact: 4 significant bits times a power of two)
+__device__ __forceinline__ void decode8(u32x2_u c, unsigned scale_byte, float (&v)[8]) {
+  const float f = pow2f((int)scale_byte - 127);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    v[4 * h] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 0) * f;
+    v[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 1) * f;
+    v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 2) * f;
+    v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 3) * f;
+  }
+}
+
+__device__ __forceinline__ u32x2_u load_codes(const uint8_t* __restrict__ p, int n) {
+  u32x2_u c;
+  if (n >= 8) {
+    c = *reinterpret_cast<const u32x2_u*>(p);
+  } else {
+    c[0] = c[1] = 0u;
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) c[e >> 2] |= (unsigned)p[e] << (8 * (e & 3));
+  }
+  return c;
+}
+
+__device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int n, u32x2_u c) {
+  if (n >= 8) {
+    *reinterpret_cast<u32x2_u*>(p) = c;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 7; ++e)
+      if (e < n) p[e] = (uint8_t)(c[e >> 2] >> (8 * (e & 3)));
+  }
+}
+
+// sums the P lines of part [P][W] in a fixed order: columns below `split` to out0, the others to out1 (layernorm_train.hip)
+int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream);
+
+inline bool dtype_ok(int t) { return t == OVIS_F32 || t == OVIS_F16 || t == OVIS_BF16; }
+inline int dtype_size(int t) { return t == OVIS_F32 ? 4 : 2; }
+
+}  // namespace ovis

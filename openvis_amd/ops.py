@@ -4,6 +4,7 @@ torch is used for device memory, streams and shape bookkeeping only; all arithme
 the hand-written gfx950 kernels.  Every function requires CUDA(HIP) tensors and raises otherwise.
 """
 import ctypes
+import typing
 
 import torch
 
@@ -1035,3 +1036,148 @@ def gemm_nt_planes(a3, w3, bias=None, residual=None, act=ACT_NONE, out_planes=Fa
         _lib.call("ovis_gemm_nt_bf16x3_planes", a3, _ll(K), _ll(M * K), w3, _ll(K), _ll(N * K), out, _ll(N), _ll(M * N), M, N, K, bias,
                   residual, _ll(N), act, int(out_planes), _lib.stream_ptr())
     return out
+
+
+# ---- training-side operators (csrc/layernorm_train.hip, relpos.hip, act_ckpt8.hip, wgrad_ckpt8.hip; include/openvis_hip.h) --------------
+# Forward passes that keep what the backward pass needs, and the backward passes, as plain functions: they take and return tensors and
+# build no autograd graph.  f32 / fp16 / bf16 tensors, f32 arithmetic, sums in a fixed order (the same bits at every call).  Rows may be
+# strided (a slice of wider rows); the elements of a row are contiguous.  Workspaces come from torch's allocator at every call, so calls on
+# several streams, or in several captured graphs, share nothing.
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class Ckpt8(typing.NamedTuple):
+    """A matrix [rows, C] in 8 bits: codes float8_e4m3fn [rows, C] and one power-of-two scale per 32 columns, float8_e8m0fnu
+    [rows, ceil(C / 32)].  It stands for codes * scales."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class LayerNormForward(typing.NamedTuple):
+    y: torch.Tensor
+    sum: torch.Tensor            # x + residual in x's type (x itself without a residual): the rows the statistics belong to
+    stats: torch.Tensor          # f32 [rows, 2] = (mean, 1 / sqrt(var + eps))
+    xhat8: typing.Optional[Ckpt8]
+
+
+def _train_check(name, *tensors):
+    """every tensor on the current HIP device: kernels are queued on that device's current stream"""
+    cur = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == cur):
+            raise _lib.OvisError(f"{name}: tensors must be on the current HIP device (got {t.device}, current cuda:{cur}; no CPU fallback)")
+
+
+def _train_dtype(name, what, t):
+    d = _DTYPES.get(t if isinstance(t, torch.dtype) else t.dtype)
+    if d is None:
+        raise _lib.OvisError(f"{name}: {what} must be float32, float16 or bfloat16")
+    return d
+
+
+def _train_rows(name, what, t, C):
+    """(rows, row stride in elements) of t [..., C]"""
+    if t.dim() < 1 or t.shape[-1] != C or C < 1:
+        raise _lib.OvisError(f"{name}: {what} must be [..., {C}], got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.numel() // C, C
+    try:
+        v = t.view(-1, C)
+    except RuntimeError:
+        v = None
+    if v is None or (C > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < C):
+        raise _lib.OvisError(f"{name}: {what} needs contiguous elements in rows that are one stride apart (got strides {tuple(t.stride())})")
+    return v.shape[0], (v.stride(0) if v.shape[0] > 1 else C)
+
+
+def _train_vec(name, what, t, C):
+    if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
+        raise _lib.OvisError(f"{name}: {what} must be a contiguous float32 vector of {C}")
+
+
+def _train_ckpt(name, ck):
+    codes, scales = ck
+    if (codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu or codes.dim() != 2 or not codes.is_contiguous()
+            or not scales.is_contiguous() or codes.shape[1] < 1 or tuple(scales.shape) != (codes.shape[0], (codes.shape[1] + 31) // 32)):
+        raise _lib.OvisError(f"{name}: a Ckpt8 holds contiguous float8_e4m3fn codes [rows, C] and float8_e8m0fnu scales [rows, ceil(C / 32)]")
+    return codes.shape
+
+
+def _ptr(t):
+    return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
+
+
+def _new_ckpt(rows, C, device):
+    return Ckpt8(torch.empty((rows, C), dtype=torch.float8_e4m3fn, device=device),
+                 torch.empty((rows, (C + 31) // 32), dtype=torch.float8_e8m0fnu, device=device))
+
+
+def layernorm_forward(x, gamma, beta, residual=None, eps=1e-5, out_dtype=None, checkpoint=False):
+    """layernorm() for training: x [..., C] (+ residual of the same shape and type) -> LayerNormForward(y, sum, stats, xhat8).
+    y has out_dtype (x's type, or any of the three where x is f32); checkpoint=True also keeps the normalised rows in 8 bits, from which
+    layernorm_backward and linear_wgrad_ckpt8 work without x.  C <= 8192.  The reference trains nn.LayerNorm, msdeformattn.py:139-146."""
+    name = "layernorm_forward"
+    C = x.shape[-1] if x.dim() else 0
+    _train_check(name, x, gamma, beta, residual)
+    xd = _train_dtype(name, "x", x)
+    yd = xd if out_dtype is None else _train_dtype(name, "out_dtype", out_dtype)
+    rows, ldx = _train_rows(name, "x", x, C)
+    ldr = 0
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != x.shape:
+            raise _lib.OvisError(f"{name}: residual must have x's shape and type")
+        ldr = _train_rows(name, "residual", residual, C)[1]
+    _train_vec(name, "gamma", gamma, C)
+    _train_vec(name, "beta", beta, C)
+    y = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else x
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    ck = _new_ckpt(rows, C, x.device) if checkpoint else None
+    if rows:
+        _lib.call("ovis_layernorm_train_forward", _ptr(x), _ll(ldx), _ptr(residual), _ll(ldr), gamma, beta, _ptr(total if residual is not None else None),
+                  y, stats, _ptr(ck.codes if ck else None), _ptr(ck.scales if ck else None), _ll(rows), C, ctypes.c_float(eps), xd, yd, _lib.stream_ptr())
+    return LayerNormForward(y, total, stats, ck)
+
+
+def layernorm_backward(dy, x, stats, gamma, dsum=None, out_dtype=None):
+    """Gradients of layernorm_forward: (dx, dgamma, dbeta), dgamma / dbeta in f32.  x: the rows that were normalised (`sum`), or `xhat8`; dsum: the
+    gradient that reaches those rows past the norm, added to dx.  dx has out_dtype (default: x's type, or dsum's, or dy's with an 8-bit x)."""
+    name = "layernorm_backward"
+    ck = x if isinstance(x, Ckpt8) else None
+    C = dy.shape[-1] if dy.dim() else 0
+    _train_check(name, dy, stats, gamma, dsum, *(ck if ck else (x,)))
+    dyd = _train_dtype(name, "dy", dy)
+    rows, lddy = _train_rows(name, "dy", dy, C)
+    ldx = 0
+    if ck is not None:
+        if tuple(_train_ckpt(name, ck)) != (rows, C):
+            raise _lib.OvisError(f"{name}: the 8-bit rows are {tuple(ck.codes.shape)}, dy has {rows} rows of {C}")
+        xdt = out_dtype if out_dtype is not None else dsum.dtype if dsum is not None else dy.dtype
+    else:
+        xrows, ldx = _train_rows(name, "x", x, C)
+        if xrows != rows:
+            raise _lib.OvisError(f"{name}: x has {xrows} rows, dy {rows}")
+        xdt = x.dtype
+        if out_dtype is not None and out_dtype != xdt:
+            raise _lib.OvisError(f"{name}: dx has x's type")
+    xd = _train_dtype(name, "x / dx", xdt)
+    if xd != 0 and xd != dyd:
+        raise _lib.OvisError(f"{name}: dy has dx's type, or any where dx is f32")
+    lds = 0
+    if dsum is not None:
+        srows, lds = _train_rows(name, "dsum", dsum, C)
+        if dsum.dtype != xdt or srows != rows:
+            raise _lib.OvisError(f"{name}: dsum must have dx's type and rows")
+    if stats.dtype != torch.float32 or stats.numel() != 2 * rows or not stats.is_contiguous():
+        raise _lib.OvisError(f"{name}: stats must be contiguous float32 [{rows}, 2]")
+    _train_vec(name, "gamma", gamma, C)
+    dx = torch.empty(dy.shape, dtype=xdt, device=dy.device)
+    if not rows:
+        return dx, torch.zeros((C,), dtype=torch.float32, device=dy.device), torch.zeros((C,), dtype=torch.float32, device=dy.device)
+    grads = torch.empty((2, C), dtype=torch.float32, device=dy.device)
+    wsb = _lib.lib().ovis_layernorm_train_backward_workspace_bytes(_ll(rows), C)
+    ws = torch.empty((wsb // 4,), dtype=torch.float32, device=dy.device)
+    dgamma, dbeta = grads[0], grads[1]
+    _lib.call("ovis_layernorm_train_backward", _ptr(dy), _ll(lddy), _ptr(x if ck is None else None), _ll(ldx), _ptr(ck.codes if ck else None),
+              _ptr(ck.scales if ck else None), stats, gamma, _ptr(dsum), _ll(lds), dx, dgamma, dbeta, ws, _ll(rows), C, dyd, xd, _lib.stream_ptr())
+    return dx, dgamma, dbeta

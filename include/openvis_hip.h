@@ -578,6 +578,21 @@ int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x,
                                   const float* stats, const float* gamma, const void* dsum, long long ldds, void* dx, float* dgamma,
                                   float* dbeta, float* workspace, long long rows, int C, int dy_dtype, int x_dtype, ovis_stream_t stream);
 
+/* An MLP's activation function with its input kept in 8 bits (act codes as above; the reference trains ReLU FFNs, msdeformattn.py:118-121,
+ * QuickGELU, model.py:232-234, and GELU, swin.py:21-41).
+ *   forward: y [rows, C] = act(h), codes / scales = h in 8 bits; act 0 with y NULL: the 8-bit form alone.  With ReLU the sign bit of a code
+ *     says that the value was not positive.  h, y and dy, dh have one type.
+ *   backward: dh = dy act'(value of the code), dbias f32 [C] = sum over rows of dh before its rounding (fixed order), codes_out / scales_out
+ *     (both or neither NULL) = act(value of the code) in 8 bits; workspace of ovis_act_ckpt8_backward_workspace_bytes(rows, C) bytes.
+ *   decode: out [rows, C] = the values that the codes stand for, rounded to dtype. */
+int ovis_act_ckpt8_forward(const void* h, long long ldh, void* y, uint8_t* codes, uint8_t* scales, long long rows, int C, int act, int dtype,
+                           ovis_stream_t stream);
+long long ovis_act_ckpt8_backward_workspace_bytes(long long rows, int C);
+int ovis_act_ckpt8_backward(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, void* dh, float* dbias,
+                            uint8_t* codes_out, uint8_t* scales_out, float* workspace, long long rows, int C, int act, int dtype,
+                            ovis_stream_t stream);
+int ovis_ckpt8_decode(const uint8_t* codes, const uint8_t* scales, void* out, long long rows, int C, int dtype, ovis_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

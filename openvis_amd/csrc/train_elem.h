@@ -52,35 +52,37 @@ __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v
 __device__ __forceinline__ float pow2f(int e) { return __builtin_bit_cast(float, (unsigned)(e + 127) << 23); }   // -126 <= e <= 127
 
 // maximum over the four lanes of a block (quad_perm moves inside groups of four lanes: no LDS)
-__device__ __forceinline__ float quad_max(float a) {
-  int t = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, a), 0xB1, 0xf, 0xf, true);      // lanes 1 0 3 2
-  a = fmaxf(a, __builtin_bit_cast(float, t));
-  t = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, a), 0x4E, 0xf, 0xf, true);          // lanes 2 3 0 1
-  return fmaxf(a, __builtin_bit_cast(float, t));
+__device__ __forceinline__ unsigned quad_max(unsigned a) {
+  a = max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0xB1, 0xf, 0xf, true));            // lanes 1 0 3 2
+  return max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0x4E, 0xf, 0xf, true));         // lanes 2 3 0 1
 }
+
+__device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
 // 8 values of one lane (the block's other 24 in its three neighbours; all four lanes active) -> 8 codes, and the scale's byte.
 // signed_zero: a value of 0 gets the code -0, so that a code's sign bit says "not positive" (ReLU's derivative).
+// The maximum is taken over the magnitudes' bits: they order as the values do, with infinity and then every NaN (signalling ones too, which
+// a floating-point maximum would pass on) at the top.
 __device__ __forceinline__ u32x2_u encode8(const float (&v)[8], bool signed_zero, unsigned& scale_byte) {
-  float a = 0.f;
+  constexpr unsigned kInf = 0x7f800000u;
+  unsigned a = 0u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));          // fmaxf passes a NaN over
+  for (int e = 0; e < 8; ++e) a = max(a, magnitude(v[e]));
   a = quad_max(a);
   float w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = v[e];
-  if (a == INFINITY) {                                             // rare: the maximum of the finite ones, infinities to NaN
-    a = 0.f;
+  if (a >= kInf) {                                                 // rare: the maximum of the finite ones, the others to NaN
+    a = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool inf = fabsf(w[e]) == INFINITY;
-      a = fmaxf(a, inf ? 0.f : fabsf(w[e]));
-      w[e] = inf ? NAN : w[e];
+      const bool fine = magnitude(w[e]) < kInf;
+      a = max(a, fine ? magnitude(w[e]) : 0u);
+      w[e] = fine ? w[e] : NAN;
     }
     a = quad_max(a);
   }
-  const unsigned bits = __builtin_bit_cast(unsigned, a);
-  int s = (int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);       // 1.75 * 2^8 = 448
+  int s = (int)(a >> 23) - 135 + ((a & 0x7fffffu) > 0x600000u ? 1 : 0);             // 1.75 * 2^8 = 448
   s = min(max(s, -100), 120);
   scale_byte = (unsigned)(s + 127);
   const float f = pow2f(-s);

@@ -1181,3 +1181,63 @@ def layernorm_backward(dy, x, stats, gamma, dsum=None, out_dtype=None):
     _lib.call("ovis_layernorm_train_backward", _ptr(dy), _ll(lddy), _ptr(x if ck is None else None), _ll(ldx), _ptr(ck.codes if ck else None),
               _ptr(ck.scales if ck else None), stats, gamma, _ptr(dsum), _ll(lds), dx, dgamma, dbeta, ws, _ll(rows), C, dyd, xd, _lib.stream_ptr())
     return dx, dgamma, dbeta
+
+
+def ckpt8_encode(x):
+    """x [..., C] in 8 bits, its leading dimensions as rows: Ckpt8.  Values are off by at most 2^-4 of themselves (2^-10 of the block's scale
+    below 2^-6 of it); NaN and infinities become NaN."""
+    return _act_ckpt8("ckpt8_encode", x, ACT_NONE)[1]
+
+
+def ckpt8_decode(ck, dtype=torch.float32):
+    """the values [rows, C] that a Ckpt8 stands for, in `dtype`"""
+    name = "ckpt8_decode"
+    _train_check(name, *ck)
+    rows, C = _train_ckpt(name, ck)
+    d = _train_dtype(name, "dtype", dtype)
+    out = torch.empty((rows, C), dtype=dtype, device=ck.codes.device)
+    if rows:
+        _lib.call("ovis_ckpt8_decode", _ptr(ck.codes), _ptr(ck.scales), out, _ll(rows), C, d, _lib.stream_ptr())
+    return out
+
+
+def act_forward_ckpt8(h, act):
+    """The activation of an MLP (ACT_RELU, ACT_QUICKGELU or ACT_GELU), for training: h [..., C] -> (y = act(h) in h's type, h as a Ckpt8)."""
+    if act not in (ACT_RELU, ACT_QUICKGELU, ACT_GELU):
+        raise _lib.OvisError("act_forward_ckpt8: act must be ACT_RELU, ACT_QUICKGELU or ACT_GELU")
+    return _act_ckpt8("act_forward_ckpt8", h, act)
+
+
+def _act_ckpt8(name, h, act):
+    C = h.shape[-1] if h.dim() else 0
+    _train_check(name, h)
+    d = _train_dtype(name, "input", h)
+    rows, ldh = _train_rows(name, "input", h, C)
+    y = torch.empty(h.shape, dtype=h.dtype, device=h.device) if act else None
+    ck = _new_ckpt(rows, C, h.device)
+    if rows:
+        _lib.call("ovis_act_ckpt8_forward", _ptr(h), _ll(ldh), _ptr(y), _ptr(ck.codes), _ptr(ck.scales), _ll(rows), C, int(act), d, _lib.stream_ptr())
+    return y, ck
+
+
+def act_backward_ckpt8(dy, h8, act, recompute=False):
+    """Gradient of act_forward_ckpt8: dy [..., C] and the 8-bit h -> (dh in dy's type, dbias f32 [C] = column sums of dh -- the gradient of the
+    bias of the linear layer that made h --, act(h8) as a Ckpt8 if recompute, else None: the operand of the next layer's weight gradient)."""
+    name = "act_backward_ckpt8"
+    if act not in (ACT_RELU, ACT_QUICKGELU, ACT_GELU):
+        raise _lib.OvisError(f"{name}: act must be ACT_RELU, ACT_QUICKGELU or ACT_GELU")
+    _train_check(name, dy, *h8)
+    rows, C = _train_ckpt(name, h8)
+    d = _train_dtype(name, "dy", dy)
+    drows, lddy = _train_rows(name, "dy", dy, C)
+    if drows != rows:
+        raise _lib.OvisError(f"{name}: dy has {drows} rows, the 8-bit rows are {rows}")
+    dh = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    y8 = _new_ckpt(rows, C, dy.device) if recompute else None
+    if not rows:
+        return dh, torch.zeros((C,), dtype=torch.float32, device=dy.device), y8
+    dbias = torch.empty((C,), dtype=torch.float32, device=dy.device)
+    ws = torch.empty((_lib.lib().ovis_act_ckpt8_backward_workspace_bytes(_ll(rows), C) // 4,), dtype=torch.float32, device=dy.device)
+    _lib.call("ovis_act_ckpt8_backward", _ptr(dy), _ll(lddy), _ptr(h8.codes), _ptr(h8.scales), dh, dbias, _ptr(y8.codes if y8 else None),
+              _ptr(y8.scales if y8 else None), ws, _ll(rows), C, int(act), d, _lib.stream_ptr())
+    return dh, dbias, y8

@@ -593,6 +593,25 @@ int ovis_act_ckpt8_backward(const void* dy, long long lddy, const uint8_t* codes
                             ovis_stream_t stream);
 int ovis_ckpt8_decode(const uint8_t* codes, const uint8_t* scales, void* out, long long rows, int C, int dtype, ovis_stream_t stream);
 
+/* Learned relative position bias by buckets, and the gradient of its table.
+ *   ovis_relpos_bias_1d: out [H, Nq, ld] (columns from Nk on are 0) with out[h,i,j] = table[bucket(j - i - q_offset), h], table f32
+ *     [buckets, H].  The bucket of a distance d is the number of borders <= d; borders_host: int32 [nborders] on the HOST, positive and
+ *     ascending, at most 256.  bidirectional 0: d = max(-r, 0) of r = j - i - q_offset, nborders + 1 buckets; 1: d = |r|, twice as many, the
+ *     second half for r > 0.  out at a 16-byte address, ld a multiple of 16 bytes.
+ *   ..._backward: dtable f32 [buckets, H] = sum over the batch and all (i, j) of dbias at b*bs + h*hs + i*ld + j (fixed order).
+ *   ovis_swin_relpos_bias_backward: the gradient of ovis_swin_relpos_bias_f32's table, f32 [(2 ws - 1)^2, H], from dbias at
+ *     b*bs + h*hs + i*ld + j, i, j < ws^2, ws <= 64 (swin.py:147-155; the bias is shared by all B windows).
+ *   workspaces of the ..._workspace_bytes. */
+int ovis_relpos_bias_1d(const float* table, void* out, const int* borders_host, int nborders, int bidirectional, int H, int Nq, int Nk, int ld,
+                        long long q_offset, int dtype, ovis_stream_t stream);
+long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk);
+int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace,
+                                 const int* borders_host, int nborders, int bidirectional, long long B, int H, int Nq, int Nk,
+                                 long long q_offset, int dtype, ovis_stream_t stream);
+long long ovis_swin_relpos_bias_backward_workspace_bytes(long long B, int H, int ws);
+int ovis_swin_relpos_bias_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace, long long B,
+                                   int H, int ws, int dtype, ovis_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

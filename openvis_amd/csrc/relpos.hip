@@ -1,0 +1,310 @@
+// Learned relative position bias by buckets, and the gradient of its table (gfx950).
+//
+//   sequences   bias[h, i, j] = table[bucket(j - i - q_offset), h]: the bucket of a distance is monotone in it on either side of 0, so a bucket
+//               is one run of diagonals and the host hands over the runs' borders (distances at which the next bucket begins)
+//   windows     bias[h, i, j] = table[(yi - yj + ws - 1)(2 ws - 1) + xi - xj + ws - 1, h] (forward: swin_ops.hip)
+//   gradient    dtable[b, h] = sum over the batch and all (i, j) of bucket b of dbias[., h, i, j]
+//
+// Bound by HBM: forward writes the bias once, backward reads the gradient once.  All sums are taken in a fixed order.
+#include "train_elem.h"
+
+namespace {
+
+using namespace ovis;
+
+constexpr int kMaxBuckets = 256;
+// borders of the buckets of one direction, ascending: bucket = number of borders <= distance; by value, as a kernel argument
+struct Borders { int n; int at[kMaxBuckets]; };
+
+__device__ __forceinline__ int bucket_of(long long r, const Borders& b, int both) {
+  const long long d = both ? (r < 0 ? -r : r) : (r < 0 ? -r : 0);
+  int lo = 0, hi = b.n;                                          // at[0] >= 1: bucket 0 is distance 0
+  while (lo < hi) {
+    const int m = (lo + hi) >> 1;
+    if (d >= b.at[m]) lo = m + 1;
+    else hi = m;
+  }
+  return lo + (both && r > 0 ? b.n + 1 : 0);
+}
+
+// A workgroup writes 256 V columns (V = 16 bytes) of a run of rows of one head.  Row i + 1 is row i moved one column on, so the values of all
+// its diagonals are laid out once in LDS and a lane holds its V columns in registers, takes one new value a row and moves the others on.
+template <typename T>
+__global__ void __launch_bounds__(256)
+relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders b, int both, int H, int Nq, int Nk, int ld, long long off,
+                  int rows) {
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ unsigned char raw[];
+  T* line = reinterpret_cast<T*>(raw);                           // line[k]: diagonal j - i = c0 - (i1 - 1) + k
+  const int h = blockIdx.z, i0 = blockIdx.y * rows, i1 = min(i0 + rows, Nq), c0 = blockIdx.x * 256 * V;
+  const int len = min(256 * V, ld - c0) + (i1 - i0) - 1;
+  for (int k = threadIdx.x; k < len; k += 256)
+    line[k] = (T)table[(long long)bucket_of((long long)c0 - (i1 - 1) + k - off, b, both) * H + h];
+  __syncthreads();
+  const int c = c0 + threadIdx.x * V;
+  if (c >= ld) return;                                           // ld % V == 0
+  typedef T vec __attribute__((ext_vector_type(V)));
+  vec v;
+  const T* p = line + threadIdx.x * V + (i1 - 1 - i0);           // p[e]: column c + e of row i0
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = p[e];
+  T* o = out + ((long long)h * Nq + i0) * ld + c;
+  for (int i = i0; i < i1; ++i) {
+    vec w = v;
+    if (c + V > Nk) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] = c + e < Nk ? v[e] : (T)0.f;
+    }
+    *reinterpret_cast<vec*>(o) = w;
+    o += ld;
+#pragma unroll
+    for (int e = V - 1; e > 0; --e) v[e] = v[e - 1];
+    if (i + 1 < i1) v[0] = *--p;
+  }
+}
+
+// Diagonal sums.  A wavefront owns 64 V diagonals, V neighbouring ones a lane, and walks down the rows of its share: the lane's V elements
+// of the next row lie one element on, so they are loaded as 16 bytes at any element's address and added to the same registers -- no
+// transposition, no LDS, no atomics.  A workgroup is four wavefronts on the same diagonals, rows dealt in turn; its sums are one line of the
+// workspace.  grid: (diagonal strips, row chunks x batch, heads).
+template <typename T>
+__global__ void __launch_bounds__(256)
+relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, long long B, int bper, int Nq,
+                  int Nk, int rows, int chunks) {
+  constexpr int V = 8;
+  __shared__ float buf[4][64 * V + 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int h = blockIdx.z, ck = blockIdx.y % chunks;
+  const long long b0 = (long long)(blockIdx.y / chunks) * bper, b1 = b0 + bper < B ? b0 + bper : B;
+  const int D = Nq + Nk - 1;
+  const int d0 = blockIdx.x * 64 * V;                            // diagonal index d: j = i + d - (Nq - 1)
+  const int dl = d0 + lane * V;
+  // rows that meet this strip: 0 <= i + d - (Nq - 1) < Nk for some d of it
+  const int lo = max(max(ck * rows, Nq - 1 - (d0 + 64 * V - 1)), 0), hi = min(min((ck + 1) * rows, Nq), Nk + Nq - 1 - d0);
+  float acc[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  for (long long b = b0; b < b1; ++b) {
+    const T* base = g + b * bs + (long long)h * hs;
+    for (int i = lo + wave; i < hi; i += 4) {
+      const int j = i + dl - (Nq - 1);
+      const T* p = base + (long long)i * ld + j;
+      if (j >= 0 && j + V <= Nk) {
+        float v[8];
+        load8(p, 8, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (j + e >= 0 && j + e < Nk) acc[e] += (float)p[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) buf[wave][lane * V + e] = acc[e];
+  __syncthreads();
+  float* line = part + ((long long)blockIdx.y * gridDim.z + h) * D;
+  for (int k = threadIdx.x; k < 64 * V; k += 256)
+    if (d0 + k < D) line[d0 + k] = (buf[0][k] + buf[1][k]) + (buf[2][k] + buf[3][k]);
+}
+
+// sum over a workgroup's 256 values, in a fixed order
+__device__ __forceinline__ float block_sum(float s, float* buf) {
+  buf[threadIdx.x] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) buf[threadIdx.x] += buf[threadIdx.x + o];
+    __syncthreads();
+  }
+  return buf[0];
+}
+
+// dtable[bucket, h]: the sum over the bucket's run of diagonals
+__global__ void __launch_bounds__(256)
+relpos_bwd_finish_kernel(const float* __restrict__ diag, float* __restrict__ dtable, Borders b, int both, int H, int Nq, int Nk, long long off) {
+  __shared__ float buf[256];
+  const int bk = blockIdx.x, h = blockIdx.y, D = Nq + Nk - 1, side = b.n + 1;
+  // the bucket's r = j - i - off, as a run [r0, r1)
+  const bool pos = both && bk >= side;
+  const int k = pos ? bk - side : bk;
+  const long long far = 1ll << 61, first = k == 0 ? 0 : b.at[k - 1], last = k == b.n ? far : b.at[k];      // magnitudes [first, last)
+  const long long r0 = pos ? (first > 1 ? first : 1) : 1 - last;
+  const long long r1 = pos ? last : k == 0 && !both ? far : 1 - first;                                     // one direction: r > 0 is distance 0 too
+  const long long shift = (long long)(Nq - 1) + off;
+  const long long d0 = min(max(r0 + shift, 0ll), (long long)D), d1 = min(max(r1 + shift, 0ll), (long long)D);
+  float s = 0.f;
+  for (long long d = d0 + threadIdx.x; d < d1; d += 256) s += diag[(long long)h * D + d];
+  s = block_sum(s, buf);
+  if (threadIdx.x == 0) dtable[(long long)bk * H + h] = s;
+}
+
+// Windows: sum over a run of the batch, element by element (grid: pieces of the [H, N, N] plane, batch chunks), then over the pairs of each
+// bucket.
+template <typename T>
+__global__ void __launch_bounds__(256)
+window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, int H, int N, int nvec,
+                       long long B, long long chunk) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)H * N * nvec) return;
+  const int v = (int)(i % nvec);
+  const long long hr = i / nvec;
+  const int row = (int)(hr % N), h = (int)(hr / N), n = N - v * 8;
+  const long long b0 = (long long)blockIdx.y * chunk, b1 = b0 + chunk < B ? b0 + chunk : B;
+  const T* p = g + h * hs + row * ld + v * 8;
+  float acc[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (long long b = b0; b < b1; ++b) {
+    float x[8];
+    load8(p + b * bs, n, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += x[e];
+  }
+  store8(part + (((long long)blockIdx.y * H + h) * N + row) * N + v * 8, n, acc);
+}
+
+__global__ void __launch_bounds__(256)
+window_bias_finish_kernel(const float* __restrict__ sum, float* __restrict__ dtable, int H, int ws) {
+  __shared__ float buf[256];
+  const int bk = blockIdx.x, h = blockIdx.y, N = ws * ws, w = 2 * ws - 1;
+  const int dy = bk / w - (ws - 1), dx = bk % w - (ws - 1);      // yi - yj, xi - xj
+  const int ny = ws - abs(dy), nx = ws - abs(dx), n = ny * nx;
+  float s = 0.f;
+  for (int t = threadIdx.x; t < n; t += 256) {
+    const int yj = max(0, -dy) + t / nx, xj = max(0, -dx) + t % nx;
+    s += sum[((long long)h * N + (yj + dy) * ws + xj + dx) * N + yj * ws + xj];
+  }
+  s = block_sum(s, buf);
+  if (threadIdx.x == 0) dtable[(long long)bk * H + h] = s;
+}
+
+// Workgroups: about sixteen a CU; a long sequence's rows are split (32 at least a workgroup), a large batch's entries go several to one.
+struct SeqShape { int strips, chunks, rows, bper; long long lines; };
+inline SeqShape seq_shape(long long B, int H, int Nq, int Nk) {
+  SeqShape s;
+  s.strips = (int)(((long long)Nq + Nk - 1 + 511) / 512);
+  const long long per = B * H * s.strips;
+  long long want = (4096 + per - 1) / per;
+  const long long most = (Nq + 31) / 32;
+  if (want > most) want = most;
+  s.rows = (int)((Nq + want - 1) / want);
+  s.chunks = (Nq + s.rows - 1) / s.rows;
+  s.bper = (int)(per > 4096 ? (per + 4095) / 4096 : 1);
+  s.lines = (B + s.bper - 1) / s.bper * s.chunks;
+  return s;
+}
+struct WinShape { long long chunk; int chunks; };
+inline WinShape win_shape(long long B, int H, int N) {
+  const long long blocks = ((long long)H * N * ((N + 7) / 8) + 255) / 256;
+  long long want = (2048 + blocks - 1) / blocks;
+  const long long most = (B + 3) / 4;
+  if (want > most) want = most;
+  if (want > 65535) want = 65535;
+  WinShape s;
+  s.chunk = (B + want - 1) / want;
+  s.chunks = (int)((B + s.chunk - 1) / s.chunk);
+  return s;
+}
+
+inline int fill_borders(Borders& b, const int* borders_host, int n) {
+  if (n < 0 || n > kMaxBuckets || (n && !borders_host)) return fail(OVIS_EINVAL, "relpos_bias: 0 to %d borders", kMaxBuckets);
+  b.n = n;
+  for (int i = 0; i < n; ++i) {
+    b.at[i] = borders_host[i];
+    if (b.at[i] < 1 || (i && b.at[i] < b.at[i - 1])) return fail(OVIS_EINVAL, "relpos_bias: borders must be positive and ascending");
+  }
+  return OVIS_OK;
+}
+
+}  // namespace
+
+#define RP_TYPE(dtype, CALL)                         \
+  if (dtype == OVIS_F32) { CALL(float) }             \
+  else if (dtype == OVIS_F16) { CALL(_Float16) }     \
+  else { CALL(__bf16) }
+
+extern "C" int ovis_relpos_bias_1d(const float* table, void* out, const int* borders_host, int nborders, int bidirectional, int H, int Nq, int Nk,
+                                   int ld, long long q_offset, int dtype, ovis_stream_t stream) {
+  OVIS_REQUIRE(table && out && ovis::dtype_ok(dtype), "relpos_bias_1d: null pointer or type %d", dtype);
+  OVIS_REQUIRE(H > 0 && H <= 65535 && Nq > 0 && Nk > 0 && Nq < (1 << 30) && Nk < (1 << 30) && q_offset < (1ll << 60) && q_offset > -(1ll << 60),
+               "relpos_bias_1d: H %d, Nq %d, Nk %d", H, Nq, Nk);
+  OVIS_REQUIRE(ld >= Nk && ld % (16 / ovis::dtype_size(dtype)) == 0 && ((uintptr_t)out & 15) == 0,
+               "relpos_bias_1d: rows of 16-byte multiples at 16-byte addresses");
+  Borders b;
+  const int rc = fill_borders(b, borders_host, nborders);
+  if (rc != OVIS_OK) return rc;
+  const int cols = 256 * 16 / ovis::dtype_size(dtype);
+  const unsigned strips = ovis::cdiv(ld, cols);
+  int rows = 64;
+  while ((long long)((Nq + rows - 1) / rows) > 65535) rows *= 2;
+  OVIS_REQUIRE(rows <= 16384, "relpos_bias_1d: too many rows");
+#define RP_GO(T)                                                                                                                            \
+  hipLaunchKernelGGL((relpos_fwd_kernel<T>), dim3(strips, (Nq + rows - 1) / rows, H), dim3(256), (cols + rows) * sizeof(T),                 \
+                     (hipStream_t)stream, table, (T*)out, b, bidirectional, H, Nq, Nk, ld, q_offset, rows);
+  RP_TYPE(dtype, RP_GO)
+#undef RP_GO
+  return ovis::check_launch("relpos_bias_1d");
+}
+
+extern "C" long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk) {
+  if (B <= 0 || H <= 0 || Nq <= 0 || Nk <= 0) return 0;
+  return (seq_shape(B, H, Nq, Nk).lines + 1) * H * ((long long)Nq + Nk - 1) * 4;
+}
+
+extern "C" int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace,
+                                            const int* borders_host, int nborders, int bidirectional, long long B, int H, int Nq, int Nk,
+                                            long long q_offset, int dtype, ovis_stream_t stream) {
+  OVIS_REQUIRE(dbias && dtable && workspace && ovis::dtype_ok(dtype), "relpos_bias_1d_backward: null pointer or type %d", dtype);
+  OVIS_REQUIRE(B > 0 && H > 0 && H <= 65535 && Nq > 0 && Nk > 0 && Nq < (1 << 30) && Nk < (1 << 30) && q_offset < (1ll << 60) &&
+               q_offset > -(1ll << 60), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d", B, H, Nq, Nk);
+  OVIS_REQUIRE(ld >= 0 && bs >= 0 && hs >= 0, "relpos_bias_1d_backward: negative stride");
+  Borders b;
+  const int rc = fill_borders(b, borders_host, nborders);
+  if (rc != OVIS_OK) return rc;
+  const SeqShape s = seq_shape(B, H, Nq, Nk);
+  const long long W = (long long)H * (Nq + Nk - 1);
+  OVIS_REQUIRE(s.lines <= 65535 && W < (1ll << 31), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
+#define RP_GO(T)                                                                                                                            \
+  hipLaunchKernelGGL((relpos_bwd_kernel<T>), dim3(s.strips, (unsigned)s.lines, H), dim3(256), 0, (hipStream_t)stream, (const T*)dbias, bs,  \
+                     hs, ld, workspace + W, B, s.bper, Nq, Nk, s.rows, s.chunks);
+  RP_TYPE(dtype, RP_GO)
+#undef RP_GO
+  int rc2 = ovis::check_launch("relpos_bias_1d_backward");
+  if (rc2 == OVIS_OK && s.lines > 1)
+    rc2 = ovis::column_sum_finish(workspace + W, (int)s.lines, (int)W, workspace, (int)W, workspace, (hipStream_t)stream);
+  if (rc2 != OVIS_OK) return rc2;
+  const int buckets = (b.n + 1) * (bidirectional ? 2 : 1);
+  hipLaunchKernelGGL(relpos_bwd_finish_kernel, dim3(buckets, H), dim3(256), 0, (hipStream_t)stream, s.lines > 1 ? workspace : workspace + W,
+                     dtable, b, bidirectional, H, Nq, Nk, q_offset);
+  return ovis::check_launch("relpos_bias_1d_backward");
+}
+
+extern "C" long long ovis_swin_relpos_bias_backward_workspace_bytes(long long B, int H, int ws) {
+  if (B <= 0 || H <= 0 || ws <= 0 || ws > 64) return 0;
+  return ((long long)win_shape(B, H, ws * ws).chunks + 1) * H * ws * ws * ws * ws * 4;
+}
+
+extern "C" int ovis_swin_relpos_bias_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace,
+                                              long long B, int H, int ws, int dtype, ovis_stream_t stream) {
+  OVIS_REQUIRE(dbias && dtable && workspace && ovis::dtype_ok(dtype), "swin_relpos_bias_backward: null pointer or type %d", dtype);
+  OVIS_REQUIRE(B > 0 && H > 0 && H <= 65535 && ws > 0 && ws <= 64 && ld >= 0 && bs >= 0 && hs >= 0,
+               "swin_relpos_bias_backward: B %lld, heads %d, window %d (1 to 64)", B, H, ws);
+  const int N = ws * ws, nvec = (N + 7) / 8;
+  const WinShape s = win_shape(B, H, N);
+  const long long W = (long long)H * N * N;
+  OVIS_REQUIRE(W < (1ll << 31), "swin_relpos_bias_backward: %d heads of windows of %d are too large for one call", H, ws);
+#define RP_GO(T)                                                                                                                            \
+  hipLaunchKernelGGL((window_bias_sum_kernel<T>), dim3(ovis::cdiv((long long)H * N * nvec, 256), s.chunks), dim3(256), 0,                   \
+                     (hipStream_t)stream, (const T*)dbias, bs, hs, ld, workspace + W, H, N, nvec, B, s.chunk);
+  RP_TYPE(dtype, RP_GO)
+#undef RP_GO
+  int rc = ovis::check_launch("swin_relpos_bias_backward");
+  if (rc == OVIS_OK && s.chunks > 1)
+    rc = ovis::column_sum_finish(workspace + W, s.chunks, (int)W, workspace, (int)W, workspace, (hipStream_t)stream);
+  if (rc != OVIS_OK) return rc;
+  hipLaunchKernelGGL(window_bias_finish_kernel, dim3((2 * ws - 1) * (2 * ws - 1), H), dim3(256), 0, (hipStream_t)stream,
+                     s.chunks > 1 ? workspace : workspace + W, dtable, H, ws);
+  return ovis::check_launch("swin_relpos_bias_backward");
+}

@@ -4,6 +4,7 @@ torch is used for device memory, streams and shape bookkeeping only; all arithme
 the hand-written gfx950 kernels.  Every function requires CUDA(HIP) tensors and raises otherwise.
 """
 import ctypes
+import functools
 import typing
 
 import torch
@@ -1241,3 +1242,104 @@ def act_backward_ckpt8(dy, h8, act, recompute=False):
     _lib.call("ovis_act_ckpt8_backward", _ptr(dy), _ll(lddy), _ptr(h8.codes), _ptr(h8.scales), dh, dbias, _ptr(y8.codes if y8 else None),
               _ptr(y8.scales if y8 else None), ws, _ll(rows), C, int(act), d, _lib.stream_ptr())
     return dh, dbias, y8
+
+
+@functools.lru_cache(maxsize=64)
+def _relpos_borders(num_buckets, max_distance, bidirectional):
+    """distances at which the buckets of a direction begin (bucket 0 is distance 0), counted in whole numbers: with n = the direction's
+    buckets and e = n // 2, bucket k < e is distance k; bucket e + k begins at the first d with (d / e)^(n - e) >= (max_distance / e)^k."""
+    n = num_buckets // 2 if bidirectional else num_buckets
+    e = n // 2
+    at = list(range(1, e + 1))
+    for k in range(1, n - e):
+        lo, hi = at[-1], max_distance                 # the border is at most max_distance: (max_distance / e)^(n - e - k) >= 1
+        while lo < hi:
+            m = (lo + hi) // 2
+            if m ** (n - e) * e ** k >= max_distance ** k * e ** (n - e):
+                hi = m
+            else:
+                lo = m + 1
+        at.append(lo)
+    return (ctypes.c_int * len(at))(*at), len(at)
+
+
+def _relpos_args(name, num_buckets, max_distance, bidirectional, q_offset):
+    num_buckets, max_distance, q_offset = int(num_buckets), int(max_distance), int(q_offset)
+    n = num_buckets // 2 if bidirectional else num_buckets
+    if n < 2 or n > 257 or (bidirectional and num_buckets % 2):
+        raise _lib.OvisError(f"{name}: 2 to 257 buckets a direction, an even number in all with two directions (got {num_buckets})")
+    if not n // 2 < max_distance < 2 ** 30:
+        raise _lib.OvisError(f"{name}: max_distance must be more than the {n // 2} distances with a bucket of their own, and less than 2^30")
+    if abs(q_offset) >= 2 ** 60:
+        raise _lib.OvisError(f"{name}: q_offset {q_offset}")
+    return (*_relpos_borders(num_buckets, max_distance, bool(bidirectional)), q_offset)
+
+
+def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset=0, out_dtype=torch.float32, ld=None):
+    """Relative position bias of a sequence by buckets: table f32 [buckets, H] -> [H, Nq, Nk] with bias[h,i,j] = table[bucket(j - i - q_offset), h]
+    (a view of rows padded with zeros to 16 bytes), or with ld the padded rows themselves, [H, Nq, ld], as attention(bias=...,
+    bias_strides=(0, Nq * ld)) takes them.  A distance below half of a direction's buckets has a bucket of its own; the others grow logarithmically up to max_distance, the last bucket
+    holds all that is farther.  bidirectional: the second half of the buckets is for keys behind the query (j > i + q_offset); otherwise
+    those have distance 0.  q_offset: position of the first query among the keys (one new token of a cache: Nq = 1, q_offset = Nk - 1)."""
+    name = "relpos_bias_1d"
+    _train_check(name, table)
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.shape[1] < 1:
+        raise _lib.OvisError(f"{name}: table must be contiguous float32 [buckets, heads]")
+    borders, nb, off = _relpos_args(name, table.shape[0], max_distance, bidirectional, q_offset)
+    d = _train_dtype(name, "out_dtype", out_dtype)
+    Nq, Nk, H = int(Nq), int(Nk), table.shape[1]
+    if Nq < 0 or Nk < 0:
+        raise _lib.OvisError(f"{name}: Nq {Nq}, Nk {Nk}")
+    v = 4 if d == 0 else 8
+    row = (Nk + v - 1) // v * v if ld is None else int(ld)
+    if row < Nk or row % v:
+        raise _lib.OvisError(f"{name}: ld must be at least {Nk} and a multiple of {v}")
+    out = torch.empty((H, Nq, row), dtype=out_dtype, device=table.device)
+    if Nq and Nk:
+        _lib.call("ovis_relpos_bias_1d", table, out, borders, nb, int(bool(bidirectional)), H, Nq, Nk, row, _ll(off), d, _lib.stream_ptr())
+    elif row:
+        out.zero_()
+    return out if ld is not None or row == Nk else out[..., :Nk]
+
+
+def _relpos_grad(name, dbias):
+    """dbias [H, Nq, Nk] or [B, H, Nq, Nk] with contiguous elements -> (B, H, Nq, Nk, strides, type)"""
+    _train_check(name, dbias)
+    d = _train_dtype(name, "dbias", dbias)
+    g = dbias[None] if dbias.dim() == 3 else dbias
+    if g.dim() != 4 or g.shape[1] < 1 or (g.shape[3] > 1 and g.stride(3) != 1):
+        raise _lib.OvisError(f"{name}: dbias must be [H, Nq, Nk] or [B, H, Nq, Nk] with contiguous rows (got {tuple(dbias.shape)}, strides {tuple(dbias.stride())})")
+    return (*g.shape, *(_ll(s) for s in g.stride()[:3]), d)
+
+
+def relpos_bias_1d_backward(dbias, num_buckets, max_distance=128, bidirectional=True, q_offset=0):
+    """Gradient of relpos_bias_1d's table, f32 [num_buckets, H]: dbias [H, Nq, Nk] or [B, H, Nq, Nk] (the bias is shared by the batch; f32, fp16
+    or bf16, any strides but the last) summed over the batch and over the pairs of each bucket."""
+    name = "relpos_bias_1d_backward"
+    B, H, Nq, Nk, bs, hs, ld, d = _relpos_grad(name, dbias)
+    borders, nb, off = _relpos_args(name, num_buckets, max_distance, bidirectional, q_offset)
+    if not (B and Nq and Nk):
+        return torch.zeros((num_buckets, H), dtype=torch.float32, device=dbias.device)
+    out = torch.empty((num_buckets, H), dtype=torch.float32, device=dbias.device)
+    ws = torch.empty((_lib.lib().ovis_relpos_bias_1d_backward_workspace_bytes(_ll(B), H, Nq, Nk) // 4,), dtype=torch.float32, device=dbias.device)
+    _lib.call("ovis_relpos_bias_1d_backward", _ptr(dbias), bs, hs, ld, out, ws, borders, nb, int(bool(bidirectional)), _ll(B), H, Nq, Nk, _ll(off), d,
+              _lib.stream_ptr())
+    return out
+
+
+def swin_relpos_bias_backward(dbias, ws):
+    """Gradient of swin_relpos_bias's table, f32 [(2 ws - 1)^2, heads]: dbias [heads, N, >= N] or [B, heads, N, >= N] (N = ws * ws; columns from N
+    on are padding and not read), summed over the B windows and over the token pairs of each offset (swin.py:147-155)."""
+    name = "swin_relpos_bias_backward"
+    ws = int(ws)
+    if not 1 <= ws <= 64:
+        raise _lib.OvisError(f"{name}: window size {ws} (1 to 64)")
+    B, H, N, ld_cols, bs, hs, ld, d = _relpos_grad(name, dbias)
+    if N != ws * ws or ld_cols < N:
+        raise _lib.OvisError(f"{name}: dbias must be [..., {ws * ws}, at least {ws * ws}], got {tuple(dbias.shape)}")
+    if not B:
+        return torch.zeros(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
+    out = torch.empty(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
+    work = torch.empty((_lib.lib().ovis_swin_relpos_bias_backward_workspace_bytes(_ll(B), H, ws) // 4,), dtype=torch.float32, device=dbias.device)
+    _lib.call("ovis_swin_relpos_bias_backward", _ptr(dbias), bs, hs, ld, out, work, _ll(B), H, ws, d, _lib.stream_ptr())
+    return out

@@ -42,7 +42,8 @@ def lib():
         for fn in ("ovis_attention_workspace_bytes", "ovis_hungarian_link_workspace_bytes", "ovis_clip_crop_workspace_bytes",
                    "ovis_attention_partial_floats", "ovis_attention_partial_workspace_bytes",
                    "ovis_layernorm_train_backward_workspace_bytes", "ovis_act_ckpt8_backward_workspace_bytes",
-                   "ovis_relpos_bias_1d_backward_workspace_bytes", "ovis_swin_relpos_bias_backward_workspace_bytes"):
+                   "ovis_relpos_bias_1d_backward_workspace_bytes", "ovis_swin_relpos_bias_backward_workspace_bytes",
+                   "ovis_linear_wgrad_ckpt8_workspace_bytes"):
             if hasattr(_lib, fn):
                 getattr(_lib, fn).restype = ctypes.c_longlong
     return _lib

@@ -1343,3 +1343,29 @@ def swin_relpos_bias_backward(dbias, ws):
     work = torch.empty((_lib.lib().ovis_swin_relpos_bias_backward_workspace_bytes(_ll(B), H, ws) // 4,), dtype=torch.float32, device=dbias.device)
     _lib.call("ovis_swin_relpos_bias_backward", _ptr(dbias), bs, hs, ld, out, work, _ll(B), H, ws, d, _lib.stream_ptr())
     return out
+
+
+def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
+    """Gradients of a linear layer's weight [N, K] and bias [N] (f32): dy [..., N] and the layer's input as a Ckpt8 [rows, K] -> (dw, db).  With a
+    layer norm's gamma / beta [K], x8 is its xhat8 and the layer's input was xhat * gamma + beta."""
+    name = "linear_wgrad_ckpt8"
+    N = dy.shape[-1] if dy.dim() else 0
+    _train_check(name, dy, *x8, gamma, beta)
+    rows, K = _train_ckpt(name, x8)
+    d = _train_dtype(name, "dy", dy)
+    drows, lddy = _train_rows(name, "dy", dy, N)
+    if drows != rows:
+        raise _lib.OvisError(f"{name}: dy has {drows} rows, the 8-bit rows are {rows}")
+    if (gamma is None) != (beta is None):
+        raise _lib.OvisError(f"{name}: gamma and beta go together")
+    if gamma is not None:
+        _train_vec(name, "gamma", gamma, K)
+        _train_vec(name, "beta", beta, K)
+    if not rows:
+        return torch.zeros((N, K), dtype=torch.float32, device=dy.device), torch.zeros((N,), dtype=torch.float32, device=dy.device)
+    dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
+    db = torch.empty((N,), dtype=torch.float32, device=dy.device)
+    ws = torch.empty((_lib.lib().ovis_linear_wgrad_ckpt8_workspace_bytes(_ll(rows), N, K, d) // 4,), dtype=torch.float32, device=dy.device)
+    _lib.call("ovis_linear_wgrad_ckpt8", _ptr(dy), _ll(lddy), _ptr(x8.codes), _ptr(x8.scales), gamma, beta, dw, db, ws, _ll(rows), N, K, d,
+              _lib.stream_ptr())
+    return dw, db

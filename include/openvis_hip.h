@@ -569,11 +569,11 @@ int ovis_pil_resize_preprocess_u8(const uint8_t* src, int H, int W, uint8_t* tmp
  *     y_dtype = x_dtype, or any where x is f32; C <= 8192.
  *   backward: dx = rstd (dy gamma - mean(dy gamma) - xhat mean(dy gamma xhat)) + dsum (NULL: none), dgamma = sum dy xhat, dbeta = sum dy
  *     (fixed order: the same bits at every call); xhat from x [rows, ldx] and stats, or from codes / scales (x NULL; the mean is not used).
- *     dx and dsum have x_dtype; workspace of ovis_layernorm_train_backward_workspace_bytes(rows, C) bytes. */
+ *     dx and dsum have x_dtype; workspace of ovis_layernorm_train_backward_workspace_bytes(rows, C, x_dtype) bytes. */
 int ovis_layernorm_train_forward(const void* x, long long ldx, const void* residual, long long ldr, const float* gamma, const float* beta,
                                  void* sum, void* y, float* stats, uint8_t* codes, uint8_t* scales, long long rows, int C, float eps,
                                  int x_dtype, int y_dtype, ovis_stream_t stream);
-long long ovis_layernorm_train_backward_workspace_bytes(long long rows, int C);
+long long ovis_layernorm_train_backward_workspace_bytes(long long rows, int C, int x_dtype);
 int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x, long long ldx, const uint8_t* codes, const uint8_t* scales,
                                   const float* stats, const float* gamma, const void* dsum, long long ldds, void* dx, float* dgamma,
                                   float* dbeta, float* workspace, long long rows, int C, int dy_dtype, int x_dtype, ovis_stream_t stream);

@@ -40,10 +40,7 @@ def lib():
         _lib.ovis_last_error.restype = ctypes.c_char_p
         _lib.ovis_abi_version.restype = ctypes.c_int
         for fn in ("ovis_attention_workspace_bytes", "ovis_hungarian_link_workspace_bytes", "ovis_clip_crop_workspace_bytes",
-                   "ovis_attention_partial_floats", "ovis_attention_partial_workspace_bytes",
-                   "ovis_layernorm_train_backward_workspace_bytes", "ovis_act_ckpt8_backward_workspace_bytes",
-                   "ovis_relpos_bias_1d_backward_workspace_bytes", "ovis_swin_relpos_bias_backward_workspace_bytes",
-                   "ovis_linear_wgrad_ckpt8_workspace_bytes"):
+                   "ovis_attention_partial_floats", "ovis_attention_partial_workspace_bytes"):
             if hasattr(_lib, fn):
                 getattr(_lib, fn).restype = ctypes.c_longlong
     return _lib
@@ -103,6 +100,29 @@ def call(name, *args):
         _throttle()
 
 
+_ENTRIES = {}
+_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+
+
+def entry(name, signature, returns="i"):
+    """The ovis_* function `name` with declared argument types (p pointer, i int, l long long, f float), made once: it takes plain ints (None = a
+    null pointer), which costs a small call a few microseconds less than converting argument by argument."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        proto = ctypes.CFUNCTYPE(_CTYPES[returns], *[_CTYPES[c] for c in signature])      # a prototype of its own: call() leaves types open
+        fn = _ENTRIES[name] = proto((name, lib()))
+    return fn
+
+
+def run(name, signature, *args):
+    """entry(name, signature)(*args); raise OvisError on a non-zero code."""
+    rc = entry(name, signature)(*args)
+    if rc != 0:
+        raise OvisError(f"{name} failed (code {rc}): {lib().ovis_last_error().decode()}")
+    if LAUNCH_WINDOW > 0:
+        _throttle()
+
+
 _raw_stream = None
 
 
@@ -119,3 +139,10 @@ def stream_ptr():
         else:                                                       # other torch builds: the public, slower path
             _raw_stream = lambda: torch.cuda.current_stream().cuda_stream
     return ctypes.c_void_p(_raw_stream())
+
+
+def raw_stream():
+    """stream_ptr() as an int, for entry()"""
+    if _raw_stream is None:
+        stream_ptr()
+    return _raw_stream()

@@ -84,20 +84,30 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
+  constexpr int U = 4;                                           // rows in flight
   for (long long b = b0; b < b1; ++b) {
     const T* base = g + b * bs + (long long)h * hs;
-    for (int i = lo + wave; i < hi; i += 4) {
-      const int j = i + dl - (Nq - 1);
-      const T* p = base + (long long)i * ld + j;
-      if (j >= 0 && j + V <= Nk) {
-        float v[8];
-        load8(p, 8, v);
+    for (int i = lo + wave; i < hi; i += 4 * U) {
+      Raw8<T> v[U];
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += v[e];
-      } else {
+      for (int u = 0; u < U; ++u) {                              // a lane whose columns cross an end of the row reads them one by one, below
+        const int r = i + 4 * u, j = r + dl - (Nq - 1);
+        v[u].load_all(base + (long long)r * ld + j, r < hi && j >= 0 && j + V <= Nk);
+      }
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (j + e >= 0 && j + e < Nk) acc[e] += (float)p[e];
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += v[u].at(e);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = i + 4 * u, j = r + dl - (Nq - 1);
+        if (r < hi && ((j < 0 && j + V > 0) || (j < Nk && j + V > Nk))) {
+          const T* p = base + (long long)r * ld + j;
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (j + e >= 0 && j + e < Nk) acc[e] += (float)p[e];
+        }
       }
     }
   }

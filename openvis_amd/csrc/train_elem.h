@@ -35,6 +35,33 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)
   }
 }
 
+// the same, kept in the stored type
+template <typename T>
+struct Raw8 {
+  typename Vec8Of<T>::type v;
+  __device__ __forceinline__ void load(const T* __restrict__ p, int n) {
+    if (n >= 8) {
+      v = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void load_all(const T* __restrict__ p, bool any) {       // all eight, or none
+    v = (typename Vec8Of<T>::type)0;
+    if (any) v = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
+  }
+  __device__ __forceinline__ float at(int e) const { return (float)v[e]; }
+  // the compiler takes the registers as new from here on, so that it widens them again where they are used instead of keeping both forms
+  __device__ __forceinline__ void hide() {
+    typedef unsigned words __attribute__((ext_vector_type(sizeof(v) / 4)));
+    words w = __builtin_bit_cast(words, v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("" : "+v"(w[i]));
+    v = __builtin_bit_cast(typename Vec8Of<T>::type, w);
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void store8(T* __restrict__ p, int n, const float (&v)[8]) {
   if (n >= 8) {
@@ -108,6 +135,12 @@ __device__ __forceinline__ void decode8(u32x2_u c, unsigned scale_byte, float (&
     v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 2) * f;
     v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[h], 3) * f;
   }
+}
+
+__device__ __forceinline__ void hide(u32x2_u& c) {
+  unsigned a = c[0], b = c[1];
+  asm volatile("" : "+v"(a), "+v"(b));
+  c[0] = a, c[1] = b;
 }
 
 __device__ __forceinline__ u32x2_u load_codes(const uint8_t* __restrict__ p, int n) {

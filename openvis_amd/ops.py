@@ -1063,10 +1063,14 @@ class LayerNormForward(typing.NamedTuple):
 
 def _train_check(name, *tensors):
     """every tensor on the current HIP device: kernels are queued on that device's current stream"""
-    cur = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    cur = None
     for t in tensors:
-        if t is not None and not (t.is_cuda and t.device.index == cur):
-            raise _lib.OvisError(f"{name}: tensors must be on the current HIP device (got {t.device}, current cuda:{cur}; no CPU fallback)")
+        if t is not None:
+            d = t.get_device()
+            if cur is None:
+                cur = torch.cuda.current_device() if d >= 0 else -1
+            if d < 0 or d != cur:
+                raise _lib.OvisError(f"{name}: tensors must be on the current HIP device (got {t.device}; no CPU fallback)")
 
 
 def _train_dtype(name, what, t):
@@ -1105,7 +1109,12 @@ def _train_ckpt(name, ck):
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr() if t is not None else 0)
+    return None if t is None else t.data_ptr()
+
+
+def _workspace(name, signature, device, *args):
+    """f32 workspace of the size that the library asks for"""
+    return torch.empty((_lib.entry(name, signature, "l")(*args) // 4,), dtype=torch.float32, device=device)
 
 
 def _new_ckpt(rows, C, device):
@@ -1135,8 +1144,9 @@ def layernorm_forward(x, gamma, beta, residual=None, eps=1e-5, out_dtype=None, c
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
     ck = _new_ckpt(rows, C, x.device) if checkpoint else None
     if rows:
-        _lib.call("ovis_layernorm_train_forward", _ptr(x), _ll(ldx), _ptr(residual), _ll(ldr), gamma, beta, _ptr(total if residual is not None else None),
-                  y, stats, _ptr(ck.codes if ck else None), _ptr(ck.scales if ck else None), _ll(rows), C, ctypes.c_float(eps), xd, yd, _lib.stream_ptr())
+        _lib.run("ovis_layernorm_train_forward", "plplppppppplifiip", x.data_ptr(), ldx, _ptr(residual), ldr, gamma.data_ptr(), beta.data_ptr(),
+                 total.data_ptr() if residual is not None else None, y.data_ptr(), stats.data_ptr(), ck.codes.data_ptr() if ck else None,
+                 ck.scales.data_ptr() if ck else None, rows, C, float(eps), xd, yd, _lib.raw_stream())
     return LayerNormForward(y, total, stats, ck)
 
 
@@ -1176,11 +1186,11 @@ def layernorm_backward(dy, x, stats, gamma, dsum=None, out_dtype=None):
     if not rows:
         return dx, torch.zeros((C,), dtype=torch.float32, device=dy.device), torch.zeros((C,), dtype=torch.float32, device=dy.device)
     grads = torch.empty((2, C), dtype=torch.float32, device=dy.device)
-    wsb = _lib.lib().ovis_layernorm_train_backward_workspace_bytes(_ll(rows), C)
-    ws = torch.empty((wsb // 4,), dtype=torch.float32, device=dy.device)
-    dgamma, dbeta = grads[0], grads[1]
-    _lib.call("ovis_layernorm_train_backward", _ptr(dy), _ll(lddy), _ptr(x if ck is None else None), _ll(ldx), _ptr(ck.codes if ck else None),
-              _ptr(ck.scales if ck else None), stats, gamma, _ptr(dsum), _ll(lds), dx, dgamma, dbeta, ws, _ll(rows), C, dyd, xd, _lib.stream_ptr())
+    ws = _workspace("ovis_layernorm_train_backward_workspace_bytes", "lii", dy.device, rows, C, xd)
+    dgamma, dbeta = grads.unbind(0)
+    _lib.run("ovis_layernorm_train_backward", "plplppppplppppliiip", dy.data_ptr(), lddy, x.data_ptr() if ck is None else None, ldx,
+             ck.codes.data_ptr() if ck else None, ck.scales.data_ptr() if ck else None, stats.data_ptr(), gamma.data_ptr(), _ptr(dsum), lds,
+             dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), rows, C, dyd, xd, _lib.raw_stream())
     return dx, dgamma, dbeta
 
 
@@ -1198,7 +1208,7 @@ def ckpt8_decode(ck, dtype=torch.float32):
     d = _train_dtype(name, "dtype", dtype)
     out = torch.empty((rows, C), dtype=dtype, device=ck.codes.device)
     if rows:
-        _lib.call("ovis_ckpt8_decode", _ptr(ck.codes), _ptr(ck.scales), out, _ll(rows), C, d, _lib.stream_ptr())
+        _lib.run("ovis_ckpt8_decode", "pppliip", ck.codes.data_ptr(), ck.scales.data_ptr(), out.data_ptr(), rows, C, d, _lib.raw_stream())
     return out
 
 
@@ -1217,7 +1227,8 @@ def _act_ckpt8(name, h, act):
     y = torch.empty(h.shape, dtype=h.dtype, device=h.device) if act else None
     ck = _new_ckpt(rows, C, h.device)
     if rows:
-        _lib.call("ovis_act_ckpt8_forward", _ptr(h), _ll(ldh), _ptr(y), _ptr(ck.codes), _ptr(ck.scales), _ll(rows), C, int(act), d, _lib.stream_ptr())
+        _lib.run("ovis_act_ckpt8_forward", "plpppliiip", h.data_ptr(), ldh, _ptr(y), ck.codes.data_ptr(), ck.scales.data_ptr(), rows, C, int(act), d,
+                 _lib.raw_stream())
     return y, ck
 
 
@@ -1238,9 +1249,10 @@ def act_backward_ckpt8(dy, h8, act, recompute=False):
     if not rows:
         return dh, torch.zeros((C,), dtype=torch.float32, device=dy.device), y8
     dbias = torch.empty((C,), dtype=torch.float32, device=dy.device)
-    ws = torch.empty((_lib.lib().ovis_act_ckpt8_backward_workspace_bytes(_ll(rows), C) // 4,), dtype=torch.float32, device=dy.device)
-    _lib.call("ovis_act_ckpt8_backward", _ptr(dy), _ll(lddy), _ptr(h8.codes), _ptr(h8.scales), dh, dbias, _ptr(y8.codes if y8 else None),
-              _ptr(y8.scales if y8 else None), ws, _ll(rows), C, int(act), d, _lib.stream_ptr())
+    ws = _workspace("ovis_act_ckpt8_backward_workspace_bytes", "li", dy.device, rows, C)
+    _lib.run("ovis_act_ckpt8_backward", "plpppppppliiip", dy.data_ptr(), lddy, h8.codes.data_ptr(), h8.scales.data_ptr(), dh.data_ptr(),
+             dbias.data_ptr(), y8.codes.data_ptr() if y8 else None, y8.scales.data_ptr() if y8 else None, ws.data_ptr(), rows, C, int(act), d,
+             _lib.raw_stream())
     return dh, dbias, y8
 
 
@@ -1296,7 +1308,8 @@ def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset
         raise _lib.OvisError(f"{name}: ld must be at least {Nk} and a multiple of {v}")
     out = torch.empty((H, Nq, row), dtype=out_dtype, device=table.device)
     if Nq and Nk:
-        _lib.call("ovis_relpos_bias_1d", table, out, borders, nb, int(bool(bidirectional)), H, Nq, Nk, row, _ll(off), d, _lib.stream_ptr())
+        _lib.run("ovis_relpos_bias_1d", "pppiiiiiilip", table.data_ptr(), out.data_ptr(), borders, nb, int(bool(bidirectional)), H, Nq, Nk, row, off, d,
+                 _lib.raw_stream())
     elif row:
         out.zero_()
     return out if ld is not None or row == Nk else out[..., :Nk]
@@ -1309,7 +1322,7 @@ def _relpos_grad(name, dbias):
     g = dbias[None] if dbias.dim() == 3 else dbias
     if g.dim() != 4 or g.shape[1] < 1 or (g.shape[3] > 1 and g.stride(3) != 1):
         raise _lib.OvisError(f"{name}: dbias must be [H, Nq, Nk] or [B, H, Nq, Nk] with contiguous rows (got {tuple(dbias.shape)}, strides {tuple(dbias.stride())})")
-    return (*g.shape, *(_ll(s) for s in g.stride()[:3]), d)
+    return (*g.shape, *g.stride()[:3], d)
 
 
 def relpos_bias_1d_backward(dbias, num_buckets, max_distance=128, bidirectional=True, q_offset=0):
@@ -1321,9 +1334,9 @@ def relpos_bias_1d_backward(dbias, num_buckets, max_distance=128, bidirectional=
     if not (B and Nq and Nk):
         return torch.zeros((num_buckets, H), dtype=torch.float32, device=dbias.device)
     out = torch.empty((num_buckets, H), dtype=torch.float32, device=dbias.device)
-    ws = torch.empty((_lib.lib().ovis_relpos_bias_1d_backward_workspace_bytes(_ll(B), H, Nq, Nk) // 4,), dtype=torch.float32, device=dbias.device)
-    _lib.call("ovis_relpos_bias_1d_backward", _ptr(dbias), bs, hs, ld, out, ws, borders, nb, int(bool(bidirectional)), _ll(B), H, Nq, Nk, _ll(off), d,
-              _lib.stream_ptr())
+    ws = _workspace("ovis_relpos_bias_1d_backward_workspace_bytes", "liii", dbias.device, B, H, Nq, Nk)
+    _lib.run("ovis_relpos_bias_1d_backward", "plllpppiiliiilip", dbias.data_ptr(), bs, hs, ld, out.data_ptr(), ws.data_ptr(), borders, nb,
+             int(bool(bidirectional)), B, H, Nq, Nk, off, d, _lib.raw_stream())
     return out
 
 
@@ -1340,8 +1353,9 @@ def swin_relpos_bias_backward(dbias, ws):
     if not B:
         return torch.zeros(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
     out = torch.empty(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
-    work = torch.empty((_lib.lib().ovis_swin_relpos_bias_backward_workspace_bytes(_ll(B), H, ws) // 4,), dtype=torch.float32, device=dbias.device)
-    _lib.call("ovis_swin_relpos_bias_backward", _ptr(dbias), bs, hs, ld, out, work, _ll(B), H, ws, d, _lib.stream_ptr())
+    work = _workspace("ovis_swin_relpos_bias_backward_workspace_bytes", "lii", dbias.device, B, H, ws)
+    _lib.run("ovis_swin_relpos_bias_backward", "plllppliiip", dbias.data_ptr(), bs, hs, ld, out.data_ptr(), work.data_ptr(), B, H, ws, d,
+             _lib.raw_stream())
     return out
 
 
@@ -1365,7 +1379,7 @@ def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
         return torch.zeros((N, K), dtype=torch.float32, device=dy.device), torch.zeros((N,), dtype=torch.float32, device=dy.device)
     dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
     db = torch.empty((N,), dtype=torch.float32, device=dy.device)
-    ws = torch.empty((_lib.lib().ovis_linear_wgrad_ckpt8_workspace_bytes(_ll(rows), N, K, d) // 4,), dtype=torch.float32, device=dy.device)
-    _lib.call("ovis_linear_wgrad_ckpt8", _ptr(dy), _ll(lddy), _ptr(x8.codes), _ptr(x8.scales), gamma, beta, dw, db, ws, _ll(rows), N, K, d,
-              _lib.stream_ptr())
+    ws = _workspace("ovis_linear_wgrad_ckpt8_workspace_bytes", "liii", dy.device, rows, N, K, d)
+    _lib.run("ovis_linear_wgrad_ckpt8", "plpppppppliiip", dy.data_ptr(), lddy, x8.codes.data_ptr(), x8.scales.data_ptr(), _ptr(gamma), _ptr(beta),
+             dw.data_ptr(), db.data_ptr(), ws.data_ptr(), rows, N, K, d, _lib.raw_stream())
     return dw, db

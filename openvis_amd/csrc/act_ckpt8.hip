@@ -89,9 +89,11 @@ act_ckpt8_fwd_kernel(const T* __restrict__ h, long long ldh, T* __restrict__ y, 
 }
 
 // A workgroup owns a strip of 8 L columns and a run of rows, 256 / L of them at a time, so that a lane keeps the bias gradient of its eight
-// columns in registers; L = 64, or the next power of two where a row is shorter.
+// columns in registers; L = 64, or the next power of two where a row is shorter.  The next row is fetched while the present one is worked on, and
+// there are as many workgroups as the card holds.  73600 x 1536 fp16 GELU with the activation in 8 bits: 152 us, 4.5 TB/s (177 us without
+// either; factor and slope from an LDS table over the 512 values that codes can stand for: 162 us).
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 act_ckpt8_bwd_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                      T* __restrict__ dh, uint8_t* __restrict__ codes2, uint8_t* __restrict__ scales2, float* __restrict__ part, long long rows,
                      long long chunk, int lshift, int C) {
@@ -103,17 +105,27 @@ act_ckpt8_bwd_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  Raw8<T> dn;                                                    // the next pass's row, fetched while the present one is worked on
+  u32x2_u qn;
+  unsigned sn;
+  auto fetch = [&](long long r) {
+    const int m = r < r1 ? n : 0;
+    dn.load(dy + r * lddy + col, m);
+    qn = load_codes(codes + r * C + col, m);
+    sn = m > 0 ? scales[r * nblk + (col >> 5)] : 127u;
+  };
+  fetch(r0 + ri);
   for (long long rb = r0; rb < r1; rb += rp) {
     const long long r = rb + ri;
     const bool live = r < r1 && mine;
+    const Raw8<T> raw = dn;
+    const u32x2_u q = qn;
+    const unsigned sb0 = sn;
+    if (rb + rp < r1) fetch(r + rp);
     float h[8], d[8];
-    if (live) {
-      load8(dy + r * lddy + col, n, d);
-      decode8(load_codes(codes + r * C + col, n), scales[r * nblk + (col >> 5)], h);
-    } else {
+    decode8(q, sb0, h);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = d[e] = 0.f;
-    }
+    for (int e = 0; e < 8; ++e) d[e] = raw.at(e);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float s;
@@ -169,7 +181,7 @@ inline BwdShape bwd_shape(long long rows, int C) {
   s.strips = (unsigned)((slots + (1 << s.lshift) - 1) >> s.lshift);
   const int rp = 256 >> s.lshift;
   const long long most = (rows + rp - 1) / rp;                   // at least one pass of rows a workgroup
-  long long want = (2048 + s.strips - 1) / s.strips;             // eight workgroups a CU in all
+  long long want = s.strips < 1536 ? 1536 / s.strips : 1;        // six workgroups a CU in all: what is there at once
   if (want > most) want = most;
   s.chunk = ((rows + want - 1) / want + rp - 1) / rp * rp;
   s.chunks = (unsigned)((rows + s.chunk - 1) / s.chunk);

@@ -259,10 +259,12 @@ inline unsigned bwd_blocks(long long rows, const RowShape& s) {
 
 namespace ovis {
 
-// out0[w] (w < split), out1[w - split] = sum over the P lines of part [P][W], in a fixed order: 64 lanes of a column take every 64th line,
-// then a tree.  16 columns a workgroup: enough workgroups that the lines, which come from L2, are read in a few microseconds.
+// out0[w] (w < split), out1[w - split] = sum over the P lines of part [P][W], in a fixed order.  Two forms:
+// narrow: 64 lanes of a column take every 64th line, then a tree; 16 columns a workgroup, so that the lines, which come from L2, are read by
+// many workgroups.  wide: a lane takes four columns and all lines.  The wide form needs no exchange but fills the card only from some
+// thousands of columns on: 33 lines of 124416 columns 5 us against 20, 1024 lines of 1536 columns 60 us against 5.
 __global__ void __launch_bounds__(1024)
-column_sum_finish_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
+column_sum_narrow_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
   __shared__ float buf[64][17];
   const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4;
   const int w = blockIdx.x * 16 + c;
@@ -281,8 +283,40 @@ column_sum_finish_kernel(const float* __restrict__ part, int P, int W, float* __
   }
 }
 
+__global__ void __launch_bounds__(256)
+column_sum_wide_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
+  const long long w = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (w >= W) return;
+  typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+  f32x4_u s = {0.f, 0.f, 0.f, 0.f};
+  const int n = W - w < 4 ? (int)(W - w) : 4;
+  if (n == 4) {
+#pragma unroll 8
+    for (int p = 0; p < P; ++p) {
+      const f32x4_u t = *reinterpret_cast<const f32x4_u*>(part + (long long)p * W + w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += t[e];
+    }
+  } else {
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (e < n) s[e] += part[(long long)p * W + w + e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (e < n) {
+      if (w + e < split) out0[w + e] = s[e];
+      else out1[w + e - split] = s[e];
+    }
+  }
+}
+
 int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream) {
-  hipLaunchKernelGGL(column_sum_finish_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, part, P, W, out0, split, out1);
+  if (W >= 128 * P && W >= 16384)
+    hipLaunchKernelGGL(column_sum_wide_kernel, dim3(cdiv(W, 1024)), dim3(256), 0, stream, part, P, W, out0, split, out1);
+  else
+    hipLaunchKernelGGL(column_sum_narrow_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, part, P, W, out0, split, out1);
   return check_launch("column_sum_finish");
 }
 

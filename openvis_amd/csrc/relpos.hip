@@ -16,15 +16,15 @@ constexpr int kMaxBuckets = 256;
 // borders of the buckets of one direction, ascending: bucket = number of borders <= distance; by value, as a kernel argument
 struct Borders { int n; int at[kMaxBuckets]; };
 
-__device__ __forceinline__ int bucket_of(long long r, const Borders& b, int both) {
+__device__ __forceinline__ int bucket_of(long long r, const int* at, int n, int both) {
   const long long d = both ? (r < 0 ? -r : r) : (r < 0 ? -r : 0);
-  int lo = 0, hi = b.n;                                          // at[0] >= 1: bucket 0 is distance 0
+  int lo = 0, hi = n;                                            // at[0] >= 1: bucket 0 is distance 0
   while (lo < hi) {
     const int m = (lo + hi) >> 1;
-    if (d >= b.at[m]) lo = m + 1;
+    if (d >= at[m]) lo = m + 1;
     else hi = m;
   }
-  return lo + (both && r > 0 ? b.n + 1 : 0);
+  return lo + (both && r > 0 ? n + 1 : 0);
 }
 
 // A workgroup writes 256 V columns (V = 16 bytes) of a run of rows of one head.  Row i + 1 is row i moved one column on, so the values of all
@@ -38,8 +38,12 @@ relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders 
   T* line = reinterpret_cast<T*>(raw);                           // line[k]: diagonal j - i = c0 - (i1 - 1) + k
   const int h = blockIdx.z, i0 = blockIdx.y * rows, i1 = min(i0 + rows, Nq), c0 = blockIdx.x * 256 * V;
   const int len = min(256 * V, ld - c0) + (i1 - i0) - 1;
-  for (int k = threadIdx.x; k < len; k += 256)
-    line[k] = (T)table[(long long)bucket_of((long long)c0 - (i1 - 1) + k - off, b, both) * H + h];
+  __shared__ int at[kMaxBuckets];                                // the borders and the head's values: a search in LDS takes a fraction of one
+  __shared__ float val[2 * (kMaxBuckets + 1)];                   // through the arguments' memory
+  for (int k = threadIdx.x; k < b.n; k += 256) at[k] = b.at[k];
+  for (int k = threadIdx.x; k < (b.n + 1) * (both ? 2 : 1); k += 256) val[k] = table[(long long)k * H + h];
+  __syncthreads();
+  for (int k = threadIdx.x; k < len; k += 256) line[k] = (T)val[bucket_of((long long)c0 - (i1 - 1) + k - off, at, b.n, both)];
   __syncthreads();
   const int c = c0 + threadIdx.x * V;
   if (c >= ld) return;                                           // ld % V == 0
@@ -64,49 +68,66 @@ relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders 
 }
 
 // Diagonal sums.  A wavefront owns 64 V diagonals, V neighbouring ones a lane, and walks down the rows of its share: the lane's V elements
-// of the next row lie one element on, so they are loaded as 16 bytes at any element's address and added to the same registers -- no
-// transposition, no LDS, no atomics.  A workgroup is four wavefronts on the same diagonals, rows dealt in turn; its sums are one line of the
-// workspace.  grid: (diagonal strips, row chunks x batch, heads).
+// of the next row lie one element on, so they are loaded as one vector at any element's address and added to the same registers -- no
+// transposition, no LDS, no atomics.  A vector that crosses an end of its row is read all the same, from the neighbouring rows' elements, and
+// masked; only where it would leave the tensor's span (first and last rows) are its elements read one by one: a separate read of a row's ends
+// cost more than the rows themselves (8 x 8 x 1023^2 bf16: 50 us).  A workgroup is four wavefronts on the same diagonals, rows dealt in turn;
+// its sums are one line of the workspace.  grid: (diagonal strips, row chunks x batch, heads).
 template <typename T>
 __global__ void __launch_bounds__(256)
 relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, long long B, int bper, int Nq,
                   int Nk, int rows, int chunks) {
-  constexpr int V = 8;
+  constexpr int V = 8, U = 4;                                    // U rows in flight
   __shared__ float buf[4][64 * V + 4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.z, ck = blockIdx.y % chunks;
   const long long b0 = (long long)(blockIdx.y / chunks) * bper, b1 = b0 + bper < B ? b0 + bper : B;
+  const long long span = (B - 1) * bs + (long long)(gridDim.z - 1) * hs + (long long)(Nq - 1) * ld + Nk;
   const int D = Nq + Nk - 1;
   const int d0 = blockIdx.x * 64 * V;                            // diagonal index d: j = i + d - (Nq - 1)
-  const int dl = d0 + lane * V;
+  const int dl = d0 + lane * V - (Nq - 1);
   // rows that meet this strip: 0 <= i + d - (Nq - 1) < Nk for some d of it
   const int lo = max(max(ck * rows, Nq - 1 - (d0 + 64 * V - 1)), 0), hi = min(min((ck + 1) * rows, Nq), Nk + Nq - 1 - d0);
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
-  constexpr int U = 4;                                           // rows in flight
   for (long long b = b0; b < b1; ++b) {
-    const T* base = g + b * bs + (long long)h * hs;
+    const long long at = b * bs + (long long)h * hs;
     for (int i = lo + wave; i < hi; i += 4 * U) {
       Raw8<T> v[U];
+      const bool inside = i + d0 - (Nq - 1) >= 0 && i + 4 * (U - 1) + d0 - (Nq - 1) + 64 * V <= Nk && i + 4 * (U - 1) < hi;
+      if (inside) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {                              // a lane whose columns cross an end of the row reads them one by one, below
-        const int r = i + 4 * u, j = r + dl - (Nq - 1);
-        v[u].load_all(base + (long long)r * ld + j, r < hi && j >= 0 && j + V <= Nk);
-      }
+        for (int u = 0; u < U; ++u) v[u].load_all(g + at + (i + 4 * u) * ld + (i + 4 * u + dl), true);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int e = 0; e < V; ++e) acc[e] += v[u].at(e);
-      }
+          for (int e = 0; e < V; ++e) acc[e] += v[u].at(e);
+      } else {
+        bool alone[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = i + 4 * u, j = r + dl - (Nq - 1);
-        if (r < hi && ((j < 0 && j + V > 0) || (j < Nk && j + V > Nk))) {
-          const T* p = base + (long long)r * ld + j;
+        for (int u = 0; u < U; ++u) {
+          const int r = i + 4 * u, j = r + dl;
+          const long long o = at + r * ld + j;
+          const bool any = r < hi && j > -V && j < Nk;
+          alone[u] = any && (o < 0 || o + V > span);
+          v[u].load_all(g + o, any && !alone[u]);
+        }
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (j + e >= 0 && j + e < Nk) acc[e] += (float)p[e];
+        for (int u = 0; u < U; ++u) {
+          const int j = i + 4 * u + dl;
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += (unsigned)(j + e) < (unsigned)Nk ? v[u].at(e) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (alone[u]) {
+            const int r = i + 4 * u, j = r + dl;
+            const T* p = g + at + r * ld + j;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              if ((unsigned)(j + e) < (unsigned)Nk) acc[e] += (float)p[e];
+          }
         }
       }
     }

@@ -57,12 +57,16 @@ template <typename T> struct DyOf {                              // 8 elements o
       for (int e = 0; e < 8; ++e) v[e] = e < n ? __builtin_bit_cast(unsigned short, p[e]) : (unsigned short)0;
     }
   }
+  __device__ __forceinline__ void load_all(const T* __restrict__ p) {
+    v = __builtin_bit_cast(u16x8, *reinterpret_cast<const typename Vec8Of<T>::type*>(p));
+  }
   __device__ __forceinline__ float value(int e) const { return (float)__builtin_bit_cast(T, (unsigned short)v[e]); }
   __device__ __forceinline__ u16x8 plane(int) const { return v; }
 };
 template <> struct DyOf<float> {
   float v[8];
   __device__ __forceinline__ void load(const float* __restrict__ p, int n) { load8(p, n, v); }
+  __device__ __forceinline__ void load_all(const float* __restrict__ p) { load8(p, 8, v); }
   __device__ __forceinline__ float value(int e) const { return v[e]; }
   __device__ __forceinline__ u16x8 plane(int i) const {         // the i-th bf16 term of v (each the rest rounded to nearest)
     u16x8 r;
@@ -133,7 +137,21 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   DyOf<T> ry[YP];
   u32x2_u rx[XP];
   unsigned rs[XP];
+  const bool whole = n0 + TN <= N && k0 + TK <= K;               // no column of the tile lies outside
   auto fetch = [&](long long m) {
+    if (whole && m + BM <= m1) {
+      const T* py = dy + (m + yr) * lddy + n0 + yc;
+      const uint8_t* pc = codes + (m + xr) * K + k0 + xc;
+      const uint8_t* ps = scales + (m + xr) * nblk + ((k0 + xc) >> 5);
+#pragma unroll
+      for (int i = 0; i < YP; ++i) ry[i].load_all(py + (long long)i * YR * lddy);
+#pragma unroll
+      for (int i = 0; i < XP; ++i) {
+        rx[i] = *reinterpret_cast<const u32x2_u*>(pc + (long long)i * XR * K);
+        rs[i] = ps[(long long)i * XR * nblk];
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < YP; ++i) {
       const long long r = m + yr + i * YR;
@@ -183,15 +201,18 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   const int li = lane & 15, half = lane >> 5, colg = 16 * ((lane >> 4) & 1) + 4 * (li & 3), rowg = 8 * half + (li >> 2);
   fetch(m0);
   stage(0);
+  fetch(m0 + BM);
   __syncthreads();
   int buf = 0;
   for (long long m = m0; m < m1; m += BM) {
-    const bool more = m + BM < m1;
-    if (more) fetch(m + BM);
     const unsigned short* py = ly + buf * P * BM * TN;
     const unsigned short* px = lx + buf * BM * TK;
 #pragma unroll
     for (int st = 0; st < BM / 16; ++st) {
+      if (st == BM / 32) {                                       // halfway: the next rows into the other buffer, the ones behind them from memory
+        if (m + BM < m1) stage(buf ^ 1);
+        if (m + 2 * BM < m1) fetch(m + 2 * BM);
+      }
       u16x8 fb[AK];
 #pragma unroll
       for (int b = 0; b < AK; ++b) {
@@ -209,7 +230,6 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
           for (int b = 0; b < AK; ++b) acc[a][b] = mfma<F16>(fa, fb[b], acc[a][b]);
         }
     }
-    if (more) stage(buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }

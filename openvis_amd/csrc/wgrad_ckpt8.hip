@@ -13,6 +13,7 @@
 // All products are exact in f32; sums are f32.  Rows are split over workgroups (S parts) where there are too few tiles to fill the card; the
 // parts are added in a fixed order by a second kernel.
 #include "train_elem.h"
+#include <type_traits>
 
 namespace {
 
@@ -49,24 +50,22 @@ __device__ __forceinline__ int at(int m, int c) {
 
 template <typename T> struct DyOf {                              // 8 elements of dY as loaded
   u16x8 v;
-  __device__ __forceinline__ void load(const T* __restrict__ p, int n) {
+  __device__ __forceinline__ void load(const T* p, int n) {
     if (n >= 8) {
-      v = __builtin_bit_cast(u16x8, *reinterpret_cast<const typename Vec8Of<T>::type*>(p));
+      load_all(p);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = e < n ? __builtin_bit_cast(unsigned short, p[e]) : (unsigned short)0;
     }
   }
-  __device__ __forceinline__ void load_all(const T* __restrict__ p) {
-    v = __builtin_bit_cast(u16x8, *reinterpret_cast<const typename Vec8Of<T>::type*>(p));
-  }
+  __device__ __forceinline__ void load_all(const T* p) { v = __builtin_bit_cast(u16x8, *reinterpret_cast<const typename Vec8Of<T>::type*>(p)); }
   __device__ __forceinline__ float value(int e) const { return (float)__builtin_bit_cast(T, (unsigned short)v[e]); }
   __device__ __forceinline__ u16x8 plane(int) const { return v; }
 };
 template <> struct DyOf<float> {
   float v[8];
-  __device__ __forceinline__ void load(const float* __restrict__ p, int n) { load8(p, n, v); }
-  __device__ __forceinline__ void load_all(const float* __restrict__ p) { load8(p, 8, v); }
+  __device__ __forceinline__ void load(const float* p, int n) { load8(p, n, v); }
+  __device__ __forceinline__ void load_all(const float* p) { load8(p, 8, v); }
   __device__ __forceinline__ float value(int e) const { return v[e]; }
   __device__ __forceinline__ u16x8 plane(int i) const {         // the i-th bf16 term of v (each the rest rounded to nearest)
     u16x8 r;
@@ -100,17 +99,24 @@ __device__ __forceinline__ u16x8 widen(u32x2_u c, float f) {
   return __builtin_bit_cast(u16x8, q);
 }
 
-// TN x TK: the workgroup's tile of dW; WN x WK wavefronts; BM rows a step
+// TN x TK: the workgroup's tile of dW, on WN x WK wavefronts; BM rows a step.
+//
+// The K loop.  LDS holds three steps: one that is multiplied, the next (its first fragments are read while the last products of the present
+// one run), and one that is being written; so a step needs one barrier, and nothing waits behind it.  Registers hold three more steps on
+// their way from memory.  A step's rows are fetched without a mask: a lane whose columns lie outside the matrix reads the first ones (its products
+// go to rows or columns of dW that are not written), and one whose eight columns cross the row's end reads on into the next row; the rows
+// for which that would leave the matrix, the last ones, are done behind the loop with masks.
 template <typename T, int TN, int TK, int WN, int WK, int BM>
 __global__ void __launch_bounds__(64 * WN * WK)
 wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                    float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k) {
   constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
-  constexpr int P = sizeof(T) == 4 ? 3 : 1, NT = 64 * WN * WK, RN = TN / WN, RK = TK / WK, AN = RN / 32, AK = RK / 32;
+  constexpr int P = sizeof(T) == 4 ? 3 : 1, NT = 64 * WN * WK, RN = TN / WN, RK = TK / WK, AN = RN / 32, AK = RK / 32, NS = BM / 16;
   constexpr int YR = NT / (TN / 8), XR = NT / (TK / 8), YP = BM / YR, XP = BM / XR;        // rows a pass, passes
+  static_assert(YP * YR == BM && XP * XR == BM && YP > 0 && XP > 0, "a step is whole passes");
   extern __shared__ unsigned short lds[];
-  unsigned short* ly = lds;                                      // [2][P][BM][TN]
-  unsigned short* lx = lds + 2 * P * BM * TN;                    // [2][BM][TK]
+  unsigned short* const ly = lds;                                // [3][P][BM][TN]
+  unsigned short* const lx = lds + 3 * P * BM * TN;              // [3][BM][TK]
   __shared__ int top[TK / 32];
   const unsigned id = xcd_remap(blockIdx.x, gridDim.x);          // an XCD's workgroups: neighbouring tiles of the same rows
   const int nt = id % tiles_n, kt = (id / tiles_n) % tiles_k;
@@ -120,73 +126,70 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wn = wave / WK, wk = wave % WK;
 
   if constexpr (F16) {                                           // the largest scale of each 32 columns over the workgroup's rows
-    if (tid < TK / 32) top[tid] = 0;
+    if (tid < TK / 32) top[tid] = 27;                           // the smallest scale that the 8-bit form has
     __syncthreads();
-    const int b0 = k0 >> 5, nb = min(TK / 32, nblk - b0);
-    const int b = tid % (TK / 32);
+    const int b0 = k0 >> 5, b = tid % (TK / 32);
     int t = 0;
-    if (b < nb)
+    if (b < nblk - b0) {
+#pragma unroll 8
       for (long long m = m0 + tid / (TK / 32); m < m1; m += NT / (TK / 32)) t = max(t, (int)scales[m * nblk + b0 + b]);
+    }
     atomicMax(&top[b], t);                                       // a maximum: the order does not matter
     __syncthreads();
   }
 
   const int yr = tid / (TN / 8), yc = (tid % (TN / 8)) * 8, xr = tid / (TK / 8), xc = (tid % (TK / 8)) * 8;
-  const int yn = N - n0 - yc, xn = K - k0 - xc;
+  const int yn = N - n0 - yc, xn = K - k0 - xc;                  // columns from this lane's first on
   const int xtop = F16 ? top[xc >> 5] - 7 : 0;
-  DyOf<T> ry[YP];
-  u32x2_u rx[XP];
-  unsigned rs[XP];
-  const bool whole = n0 + TN <= N && k0 + TK <= K;               // no column of the tile lies outside
-  auto fetch = [&](long long m) {
-    if (whole && m + BM <= m1) {
-      const T* py = dy + (m + yr) * lddy + n0 + yc;
-      const uint8_t* pc = codes + (m + xr) * K + k0 + xc;
-      const uint8_t* ps = scales + (m + xr) * nblk + ((k0 + xc) >> 5);
-#pragma unroll
-      for (int i = 0; i < YP; ++i) ry[i].load_all(py + (long long)i * YR * lddy);
-#pragma unroll
-      for (int i = 0; i < XP; ++i) {
-        rx[i] = *reinterpret_cast<const u32x2_u*>(pc + (long long)i * XR * K);
-        rs[i] = ps[(long long)i * XR * nblk];
-      }
-      return;
+  struct Rows { DyOf<T> y[YP]; u32x2_u x[XP]; unsigned s[XP]; };
+  // no masks; a step's uniform row pointers and a lane's 32-bit offsets from them; in pieces, to lie between the products
+  struct At { const T* y; const uint8_t *c, *s; };
+  const unsigned oy = yr * (unsigned)lddy + (yn > 0 ? n0 + yc : 0), oc = xr * (unsigned)K + (xn > 0 ? k0 + xc : 0);
+  const unsigned os = xr * (unsigned)nblk + (xn > 0 ? (k0 + xc) >> 5 : 0);
+  auto fetch_piece = [&](Rows& R, const At& p, int i) {
+    if (i < YP) {
+      R.y[i].load_all(p.y + (long long)(i * YR) * lddy + oy);
+    } else {
+      R.x[i - YP] = *reinterpret_cast<const u32x2_u*>(p.c + (long long)((i - YP) * XR) * K + oc);
+      R.s[i - YP] = p.s[(long long)((i - YP) * XR) * nblk + os];
     }
+  };
+  auto fetch_masked = [&](Rows& R, long long m) {
 #pragma unroll
     for (int i = 0; i < YP; ++i) {
       const long long r = m + yr + i * YR;
-      ry[i].load(dy + (r < m1 ? r : m1 - 1) * lddy + n0 + (yn > 0 ? yc : 0), r < m1 ? yn : 0);
+      R.y[i].load(dy + (r < m1 ? r : m1 - 1) * lddy + n0 + (yn > 0 ? yc : 0), r < m1 ? yn : 0);
     }
 #pragma unroll
     for (int i = 0; i < XP; ++i) {
       const long long r = m + xr + i * XR;
       const bool ok = r < m1 && xn > 0;
-      rx[i][0] = rx[i][1] = 0u;
-      rs[i] = 127u;
-      if (ok) {
-        rx[i] = load_codes(codes + r * K + k0 + xc, xn);
-        rs[i] = scales[r * nblk + ((k0 + xc) >> 5)];
-      }
+      R.x[i] = load_codes(codes + (ok ? r * K + k0 + xc : 0), ok ? xn : 0);
+      R.s[i] = ok ? scales[r * nblk + ((k0 + xc) >> 5)] : 27u;
     }
   };
   float dsum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) dsum[e] = 0.f;
-  auto stage = [&](int buf) {
+  // db: every workgroup of these rows and columns n stages all of dY; they take the steps in turn
+  int turn = kt;
+  auto sum_rows = [&](const Rows& R, bool valid) {
+    if (turn == 0 && valid) {
 #pragma unroll
-    for (int i = 0; i < YP; ++i) {
+      for (int i = 0; i < YP; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dsum[e] += R.y[i].value(e);
+    }
+    turn = turn == 0 ? tiles_k - 1 : turn - 1;
+  };
+  auto stage_piece = [&](const Rows& R, int buf, int i) {
+    if (i < YP) {
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        *reinterpret_cast<u16x8*>(ly + (buf * P + p) * BM * TN + at<TN>(yr + i * YR, yc)) = ry[i].plane(p);
-      if (kt == 0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dsum[e] += ry[i].value(e);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < XP; ++i) {
-      const int e = F16 ? max((int)rs[i] - xtop, -60) : (int)rs[i] - 127;      // 60 octaves below the largest nothing is left in fp16
-      *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr + i * XR, xc)) = widen<F16>(rx[i], pow2f(e));
+        *reinterpret_cast<u16x8*>(ly + (buf * P + p) * BM * TN + at<TN>(yr + i * YR, yc)) = R.y[i].plane(p);
+    } else {
+      const int j = i - YP, e = F16 ? max((int)R.s[j] - xtop, -60) : (int)R.s[j] - 127;    // 60 octaves below the largest nothing is left in fp16
+      *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr + j * XR, xc)) = widen<F16>(R.x[j], pow2f(e));
     }
   };
 
@@ -198,40 +201,124 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
 
+  struct Frags { u16x8 a[P][AN], b[AK]; };
   const int li = lane & 15, half = lane >> 5, colg = 16 * ((lane >> 4) & 1) + 4 * (li & 3), rowg = 8 * half + (li >> 2);
-  fetch(m0);
-  stage(0);
-  fetch(m0 + BM);
-  __syncthreads();
-  int buf = 0;
-  for (long long m = m0; m < m1; m += BM) {
-    const unsigned short* py = ly + buf * P * BM * TN;
-    const unsigned short* px = lx + buf * BM * TK;
+  // fragment i of a substep: first the ones of X, then those of dY
+  auto read_piece = [&](Frags& F, int buf, int st, int i) {
+    if (i < AK) {
+      const unsigned short* q = lx + buf * BM * TK + 16 * st * TK + at<TK>(rowg, wk * RK + i * 32 + colg);
+      F.b[i] = __builtin_shufflevector(tr_read(q), tr_read(q + 4 * TK), 0, 1, 2, 3, 4, 5, 6, 7);      // 4 rows on: the same permutation
+    } else {
+      const int p = (i - AK) / AN, a = (i - AK) % AN;
+      const unsigned short* q = ly + (buf * P + p) * BM * TN + 16 * st * TN + at<TN>(rowg, wn * RN + a * 32 + colg);
+      F.a[p][a] = __builtin_shufflevector(tr_read(q), tr_read(q + 4 * TN), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  constexpr int G = P * AN, NR = AK + P * AN, NQ = YP + XP;      // groups of AK products a substep; fragments; pieces of a step's rows
+  auto multiply = [&](const Frags& F, int g) {
 #pragma unroll
-    for (int st = 0; st < BM / 16; ++st) {
-      if (st == BM / 32) {                                       // halfway: the next rows into the other buffer, the ones behind them from memory
-        if (m + BM < m1) stage(buf ^ 1);
-        if (m + 2 * BM < m1) fetch(m + 2 * BM);
+    for (int b = 0; b < AK; ++b) acc[g % AN][b] = mfma<F16>(F.a[g / AN][g % AN], F.b[b], acc[g % AN][b]);
+  };
+
+  // steps that need no mask: all their rows lie in the chunk, and what a lane reads behind a row's end lies in the matrix
+  const bool cross = (N & 7) != 0 || (K & 7) != 0;
+  const long long mf = cross && m1 > M - 8 ? (M - 8 > m0 ? M - 8 : m0) : m1;
+  const long long nf = lddy < 8 || K < 8 ? 0 : (mf - m0) / BM;
+  if (nf > 0) {
+    Rows R[3];
+    Frags F[2];
+    At next = {dy + m0 * lddy, codes + m0 * K, scales + m0 * nblk};
+    long long fetched = 0;                                       // a step of the last rows is fetched again rather than one behind them
+    auto advance = [&]() {
+      const bool more = ++fetched < nf;
+      next.y += more ? BM * lddy : 0, next.c += more ? BM * (long long)K : 0, next.s += more ? BM * (long long)nblk : 0;
+    };
+#pragma unroll
+    for (int u = 0; u < 5; ++u) {
+      if (u > 2) {
+        sum_rows(R[u - 3], u - 3 < nf);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) stage_piece(R[u - 3], u - 3, i);
       }
-      u16x8 fb[AK];
 #pragma unroll
-      for (int b = 0; b < AK; ++b) {
-        const u16x4 u = tr_read(px + at<TK>(16 * st + rowg, wk * RK + b * 32 + colg)), v = tr_read(px + at<TK>(16 * st + rowg + 4, wk * RK + b * 32 + colg));
-        fb[b] = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-#pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int a = 0; a < AN; ++a) {
-          const unsigned short* q = py + p * BM * TN;
-          const u16x4 u = tr_read(q + at<TN>(16 * st + rowg, wn * RN + a * 32 + colg)), v = tr_read(q + at<TN>(16 * st + rowg + 4, wn * RN + a * 32 + colg));
-          const u16x8 fa = __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-          for (int b = 0; b < AK; ++b) acc[a][b] = mfma<F16>(fa, fb[b], acc[a][b]);
-        }
+      for (int i = 0; i < NQ; ++i) fetch_piece(R[u % 3], next, i);
+      advance();
     }
     __syncthreads();
-    buf ^= 1;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) read_piece(F[0], 0, 0, i);
+    // step t with t % 3 == J: buffer J is multiplied, J + 1 is ready, J + 2 is written from the registers of the same number, which then take
+    // a step from memory.  The products go in groups with a share of the other work before each, in that order: left to itself the
+    // compiler puts all products of a substep behind all of its loads, and the matrix cores wait.
+    auto step = [&](long long t, auto jc, auto fc) {
+      constexpr int J = decltype(jc)::value, J1 = (J + 1) % 3, J2 = (J + 2) % 3, F0 = decltype(fc)::value;
+      sum_rows(R[J2], t + 2 < nf);
+#pragma unroll
+      for (int st = 0; st < NS; ++st) {
+        Frags &cur = F[(F0 + st) & 1], &nxt = F[(F0 + st + 1) & 1];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < NR; ++i)                           // the last group reads nothing: what it would read is needed at once
+            if (i * (G - 1) / NR == g) read_piece(nxt, st < NS - 1 ? J : J1, st < NS - 1 ? st + 1 : 0, i);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            if (st == 0 && i * G / NQ == g) stage_piece(R[J2], J2, i);
+            if (st == NS - 1 && (NS > 1 ? i * G / NQ : G - 1) == g) fetch_piece(R[J2], next, i);
+          }
+          multiply(cur, g);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      advance();
+      __syncthreads();
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    long long t = 0;
+    if constexpr (NS % 2 == 0) {
+      for (; t + 3 <= nf; t += 3) {
+        step(t, I0{}, I0{});
+        step(t + 1, I1{}, I0{});
+        step(t + 2, I2{}, I0{});
+      }
+      if (t < nf) step(t, I0{}, I0{});
+      if (t + 1 < nf) step(t + 1, I1{}, I0{});
+    } else {                                                     // an odd number of fragment sets a step: they change places every step
+      for (; t + 6 <= nf; t += 6) {
+        step(t, I0{}, I0{});
+        step(t + 1, I1{}, I1{});
+        step(t + 2, I2{}, I0{});
+        step(t + 3, I0{}, I1{});
+        step(t + 4, I1{}, I0{});
+        step(t + 5, I2{}, I1{});
+      }
+      if (t < nf) step(t, I0{}, I0{});
+      if (t + 1 < nf) step(t + 1, I1{}, I1{});
+      if (t + 2 < nf) step(t + 2, I2{}, I0{});
+      if (t + 3 < nf) step(t + 3, I0{}, I1{});
+      if (t + 4 < nf) step(t + 4, I1{}, I0{});
+    }
+  }
+  turn = (int)((kt - nf % tiles_k + tiles_k) % tiles_k);         // the steps of the loop were counted beyond its end
+  for (long long m = m0 + nf * BM; m < m1; m += BM) {
+    Rows R;
+    fetch_masked(R, m);
+    sum_rows(R, true);
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) stage_piece(R, 0, i);
+    __syncthreads();
+#pragma unroll
+    for (int st = 0; st < NS; ++st) {
+      Frags F;
+#pragma unroll
+      for (int i = 0; i < NR; ++i) read_piece(F, 0, st, i);
+#pragma unroll
+      for (int g = 0; g < G; ++g) multiply(F, g);
+    }
+    __syncthreads();
   }
 
   // a lane holds column k = lane & 31 of its blocks; register r is row (r & 3) + 8 (r >> 2) + 4 half
@@ -250,16 +337,14 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
         }
     }
   }
-  if (kt == 0) {                                                 // db: the lanes of a column group, in order
-    float* sum = reinterpret_cast<float*>(lds);                  // [YR][TN]
+  float* sum = reinterpret_cast<float*>(lds);                    // db: the lanes of a column group, in order: [YR][TN]
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[yr * TN + yc + e] = dsum[e];
-    __syncthreads();
-    for (int c = tid; c < TN; c += NT) {
-      float t = 0.f;
-      for (int i = 0; i < YR; ++i) t += sum[i * TN + c];
-      if (n0 + c < N) dbp[s * N + n0 + c] = t;
-    }
+  for (int e = 0; e < 8; ++e) sum[yr * TN + yc + e] = dsum[e];
+  __syncthreads();
+  for (int c = tid; c < TN; c += NT) {
+    float t = 0.f;
+    for (int i = 0; i < YR; ++i) t += sum[i * TN + c];
+    if (n0 + c < N) dbp[(s * tiles_k + kt) * N + n0 + c] = t;
   }
 }
 
@@ -317,7 +402,7 @@ inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
 extern "C" long long ovis_linear_wgrad_ckpt8_workspace_bytes(long long M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || !ovis::dtype_ok(dtype)) return 0;
   const WgradShape w = wgrad_shape(M, N, K, dtype);
-  return ((long long)w.S * N * K + (long long)w.S * N) * 4;
+  return ((long long)w.S * N * K + (long long)w.S * w.tiles_k * N) * 4;
 }
 
 extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, const float* gamma,
@@ -328,13 +413,15 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
                K, lddy, dtype);
   const WgradShape w = wgrad_shape(M, N, K, dtype);
   const long long blocks = (long long)w.tiles_n * w.tiles_k * w.S;
-  OVIS_REQUIRE(blocks < (1ll << 31) && (long long)N * K < (1ll << 40), "linear_wgrad_ckpt8: %d x %d is too large for one call", N, K);
+  OVIS_REQUIRE(blocks < (1ll << 31) && lddy < (1ll << 24) && K < (1 << 24), "linear_wgrad_ckpt8: %d x %d (row stride %lld) is too large for one call", N,
+               K, lddy);
   const bool join = w.S > 1 || gamma;
   float* part = join ? workspace : dw;
-  float* dbp = w.S > 1 ? workspace + (long long)w.S * N * K : db;
+  const int lines = w.S * w.tiles_k;
+  float* dbp = lines > 1 ? workspace + (long long)w.S * N * K : db;
 #define WG_GO(T, TN, TK, WN, WK, BM)                                                                                                        \
   {                                                                                                                                         \
-    const int lds = 2 * BM * (TN * (sizeof(T) == 4 ? 3 : 1) + TK) * 2;                                                                      \
+    const int lds = 3 * BM * (TN * (sizeof(T) == 4 ? 3 : 1) + TK) * 2;                                                                      \
     const hipError_t e = hipFuncSetAttribute((const void*)wgrad_ckpt8_kernel<T, TN, TK, WN, WK, BM>,                                        \
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                              \
     OVIS_REQUIRE(e == hipSuccess, "linear_wgrad_ckpt8: %s", hipGetErrorString(e));                                                          \
@@ -342,20 +429,20 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
                        (const T*)dy, lddy, codes, scales, part, dbp, M, N, K, w.chunk, w.tiles_n, w.tiles_k);                               \
   }
   if (dtype == OVIS_F32) {
-    if (w.tile == 128) WG_GO(float, 128, 128, 2, 2, 32)
+    if (w.tile == 128) WG_GO(float, 128, 128, 2, 2, 16)
     else WG_GO(float, 64, 64, 2, 2, 32)
   } else if (dtype == OVIS_F16) {
-    if (w.tile == 256) WG_GO(_Float16, 256, 256, 2, 4, 64)
-    else if (w.tile == 128) WG_GO(_Float16, 128, 128, 2, 2, 64)
-    else WG_GO(_Float16, 64, 64, 2, 2, 64)
+    if (w.tile == 256) WG_GO(_Float16, 256, 256, 2, 2, 32)
+    else if (w.tile == 128) WG_GO(_Float16, 128, 128, 2, 2, 32)
+    else WG_GO(_Float16, 64, 64, 2, 2, 32)
   } else {
-    if (w.tile == 256) WG_GO(__bf16, 256, 256, 2, 4, 64)
-    else if (w.tile == 128) WG_GO(__bf16, 128, 128, 2, 2, 64)
-    else WG_GO(__bf16, 64, 64, 2, 2, 64)
+    if (w.tile == 256) WG_GO(__bf16, 256, 256, 2, 2, 32)
+    else if (w.tile == 128) WG_GO(__bf16, 128, 128, 2, 2, 32)
+    else WG_GO(__bf16, 64, 64, 2, 2, 32)
   }
 #undef WG_GO
   int rc = ovis::check_launch("linear_wgrad_ckpt8");
-  if (rc == OVIS_OK && w.S > 1) rc = ovis::column_sum_finish(dbp, w.S, N, db, N, db, (hipStream_t)stream);
+  if (rc == OVIS_OK && lines > 1) rc = ovis::column_sum_finish(dbp, lines, N, db, N, db, (hipStream_t)stream);
   if (rc != OVIS_OK || !join) return rc;
   const long long NK = (long long)N * K;
   hipLaunchKernelGGL(wgrad_join_kernel, dim3(ovis::cdiv((NK + 3) / 4, 256)), dim3(256), 0, (hipStream_t)stream, part, w.S, db, gamma, beta, dw, NK, K);

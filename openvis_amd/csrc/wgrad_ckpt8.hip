@@ -19,6 +19,8 @@ namespace {
 
 using namespace ovis;
 
+typedef unsigned u32_u __attribute__((aligned(1)));
+typedef unsigned short u16_u __attribute__((aligned(1)));
 using f32x16 = __attribute__((ext_vector_type(16))) float;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
@@ -128,13 +130,34 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   if constexpr (F16) {                                           // the largest scale of each 32 columns over the workgroup's rows
     if (tid < TK / 32) top[tid] = 27;                           // the smallest scale that the 8-bit form has
     __syncthreads();
-    const int b0 = k0 >> 5, b = tid % (TK / 32);
-    int t = 0;
-    if (b < nblk - b0) {
+    // a lane reads a row's TK / 32 bytes at once (those behind the row's end belong to the next row, and to columns that are not used); the
+    // last rows, where that would leave the array, byte by byte
+    typedef unsigned short pairs __attribute__((ext_vector_type(2)));
+    constexpr int NB = TK / 32, NW = NB > 4 ? NB / 4 : 1;
+    const int b0 = k0 >> 5;
+    const long long whole = M - 8 < m1 ? M - 8 : m1;
+    pairs hi[NW][2];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) hi[w][0] = hi[w][1] = (pairs)0;
 #pragma unroll 8
-      for (long long m = m0 + tid / (TK / 32); m < m1; m += NT / (TK / 32)) t = max(t, (int)scales[m * nblk + b0 + b]);
+    for (long long m = m0 + tid; m < whole; m += NT) {
+      const uint8_t* p = scales + m * nblk + b0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const unsigned v = NB >= 4 ? *reinterpret_cast<const u32_u*>(p + 4 * w) : *reinterpret_cast<const u16_u*>(p);
+        hi[w][0] = __builtin_elementwise_max(hi[w][0], __builtin_bit_cast(pairs, v & 0x00ff00ffu));
+        hi[w][1] = __builtin_elementwise_max(hi[w][1], __builtin_bit_cast(pairs, (v >> 8) & 0x00ff00ffu));
+      }
     }
-    atomicMax(&top[b], t);                                       // a maximum: the order does not matter
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      int t = hi[i / 4][i & 1][(i >> 1) & 1];
+      const long long m = (whole > m0 ? whole : m0) + tid;
+      if (m < m1 && b0 + i < nblk) t = max(t, (int)scales[m * nblk + b0 + i]);
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) t = max(t, __shfl_xor(t, o, 64));
+      if (lane == 0) atomicMax(&top[i], t);                      // a maximum: the order does not matter
+    }
     __syncthreads();
   }
 
@@ -151,7 +174,8 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       R.y[i].load_all(p.y + (long long)(i * YR) * lddy + oy);
     } else {
       R.x[i - YP] = *reinterpret_cast<const u32x2_u*>(p.c + (long long)((i - YP) * XR) * K + oc);
-      R.s[i - YP] = p.s[(long long)((i - YP) * XR) * nblk + os];
+      // with the three bytes behind it: a byte's load would be widened, and so waited for, a step before it is used
+      R.s[i - YP] = *reinterpret_cast<const u32_u*>(p.s + (long long)((i - YP) * XR) * nblk + os);
     }
   };
   auto fetch_masked = [&](Rows& R, long long m) {
@@ -188,7 +212,8 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       for (int p = 0; p < P; ++p)
         *reinterpret_cast<u16x8*>(ly + (buf * P + p) * BM * TN + at<TN>(yr + i * YR, yc)) = R.y[i].plane(p);
     } else {
-      const int j = i - YP, e = F16 ? max((int)R.s[j] - xtop, -60) : (int)R.s[j] - 127;    // 60 octaves below the largest nothing is left in fp16
+      const int j = i - YP;
+      const int sb = (int)(R.s[j] & 0xffu), e = F16 ? max(sb - xtop, -60) : sb - 127;      // 60 octaves below the largest nothing is left in fp16
       *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr + j * XR, xc)) = widen<F16>(R.x[j], pow2f(e));
     }
   };
@@ -221,8 +246,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   };
 
   // steps that need no mask: all their rows lie in the chunk, and what a lane reads behind a row's end lies in the matrix
-  const bool cross = (N & 7) != 0 || (K & 7) != 0;
-  const long long mf = cross && m1 > M - 8 ? (M - 8 > m0 ? M - 8 : m0) : m1;
+  const long long mf = m1 > M - 8 ? (M - 8 > m0 ? M - 8 : m0) : m1;
   const long long nf = lddy < 8 || K < 8 ? 0 : (mf - m0) / BM;
   if (nf > 0) {
     Rows R[3];
@@ -357,6 +381,7 @@ wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict
   float v[4] = {0.f, 0.f, 0.f, 0.f};
   const int n = NK - i < 4 ? (int)(NK - i) : 4;
   typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll 4
   for (int s = 0; s < S; ++s) {
     const float* p = part + s * NK + i;
     if (n == 4) {
@@ -382,19 +407,38 @@ wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict
 }
 
 struct WgradShape { int tile, tiles_n, tiles_k, S; long long chunk; };
+// Tile and split by a model of the time (us), fitted to sweeps over shapes of 100 to 294400 rows and 8 to 4096 columns:
+//   a step of 32 rows takes `one` where a CU has one workgroup, and `more` longer for each further one, up to `most` at once; then they go in
+//   rounds.  16-bit: tile 256 1.0; 128 0.45 and 0.23; 64 0.43 and 0.22.  f32 (three products): 128 0.98 and 0.58; 64 0.45 and 0.25;
+//   S > 1 parts are written and read again at 4.5 TB/s, in a launch of its own.
+// 36928 x 1024 x 4096 fp16: tile 256 in 4 parts 328 us, 128 in 2 parts 405 us; 43120 x 512 x 512: 128 in 32 parts 55 us, 256 in 64 parts 67 us;
+// 500 x 2048 x 2048: 128 whole 21 us, 64 whole 31 us, 128 in 2 parts 33 us.
 inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
-  WgradShape w;
-  const long long t256 = (long long)cdiv(N, 256) * cdiv(K, 256), t128 = (long long)cdiv(N, 128) * cdiv(K, 128);
-  w.tile = dtype != OVIS_F32 && t256 * ((M + 1023) / 1024) >= 256 ? 256 : t128 * ((M + 511) / 512) >= 256 ? 128 : 64;
-  w.tiles_n = (int)cdiv(N, w.tile);
-  w.tiles_k = (int)cdiv(K, w.tile);
-  const long long tiles = (long long)w.tiles_n * w.tiles_k, slots = w.tile == 256 ? 256 : 512;
-  long long S = tiles >= slots ? 1 : slots / tiles;
-  const long long most = (M + 255) / 256;                        // 256 rows at least
-  if (S > most) S = most;
-  w.chunk = ((M + S - 1) / S + 63) / 64 * 64;
-  w.S = (int)((M + w.chunk - 1) / w.chunk);
-  return w;
+  WgradShape best{};
+  double least = 1e300;
+  for (int tile : {256, 128, 64}) {
+    if (tile == 256 && dtype == OVIS_F32) continue;
+    const double one = tile == 256 ? 1.0 : tile == 128 ? (dtype == OVIS_F32 ? 0.98 : 0.45) : (dtype == OVIS_F32 ? 0.45 : 0.43);
+    const double more = tile == 256 ? 0.0 : tile == 128 ? (dtype == OVIS_F32 ? 0.58 : 0.23) : (dtype == OVIS_F32 ? 0.25 : 0.22);
+    const int most = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+    const long long tn = cdiv(N, tile), tk = cdiv(K, tile), tiles = tn * tk;
+    long long last = 0;
+    for (int want : {1, 128, 256, 512, 1024}) {                  // workgroups in all
+      long long S = want / tiles, rows = (M + 63) / 64;
+      if (want > 256 * most || want == 1 || S < 1) S = 1;
+      if (S > rows) S = rows;
+      if (S == last) continue;
+      last = S;
+      const long long chunk = ((M + S - 1) / S + 31) / 32 * 32, parts = (M + chunk - 1) / chunk, wgs = tiles * parts;
+      const long long rounds = (wgs + 256 * most - 1) / (256 * most), per = wgs < 256 * most ? (wgs + 255) / 256 : most;
+      const double t = rounds * (chunk / 32) * (one + more * (per - 1)) + (parts > 1 ? 3.0 + 8.0 * parts * N * K / 4.5e6 : 0.0);
+      if (t < least) {
+        least = t;
+        best = {tile, (int)tn, (int)tk, (int)parts, chunk};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -402,7 +446,7 @@ inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
 extern "C" long long ovis_linear_wgrad_ckpt8_workspace_bytes(long long M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || !ovis::dtype_ok(dtype)) return 0;
   const WgradShape w = wgrad_shape(M, N, K, dtype);
-  return ((long long)w.S * N * K + (long long)w.S * w.tiles_k * N) * 4;
+  return ((long long)w.S * N * K + (long long)w.S * w.tiles_k * N + ((long long)N * K < 65536 ? (long long)N * K : 0)) * 4;
 }
 
 extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, const float* gamma,
@@ -445,6 +489,14 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
   if (rc == OVIS_OK && lines > 1) rc = ovis::column_sum_finish(dbp, lines, N, db, N, db, (hipStream_t)stream);
   if (rc != OVIS_OK || !join) return rc;
   const long long NK = (long long)N * K;
-  hipLaunchKernelGGL(wgrad_join_kernel, dim3(ovis::cdiv((NK + 3) / 4, 256)), dim3(256), 0, (hipStream_t)stream, part, w.S, db, gamma, beta, dw, NK, K);
+  int S = w.S;
+  if (S > 8 && NK < 65536) {                                     // few columns, many parts: 64 lanes a column (9000 x 64 x 64 in 141 parts: 57 us by one)
+    float* to = gamma ? workspace + (long long)w.S * NK + (long long)lines * N : dw;
+    rc = ovis::column_sum_finish(part, S, (int)NK, to, (int)NK, to, (hipStream_t)stream);
+    if (rc != OVIS_OK || !gamma) return rc;
+    part = to;
+    S = 1;
+  }
+  hipLaunchKernelGGL(wgrad_join_kernel, dim3(ovis::cdiv((NK + 3) / 4, 256)), dim3(256), 0, (hipStream_t)stream, part, S, db, gamma, beta, dw, NK, K);
   return ovis::check_launch("linear_wgrad_ckpt8");
 }

@@ -1112,6 +1112,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _like(t, dtype):
+    """an uninitialised contiguous tensor of t's shape (the first form costs half a microsecond less)"""
+    return torch.empty_like(t) if t.dtype == dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
+
+
 def _workspace(name, signature, device, *args):
     """f32 workspace of the size that the library asks for"""
     return torch.empty((_lib.entry(name, signature, "l")(*args) // 4,), dtype=torch.float32, device=device)
@@ -1139,9 +1144,9 @@ def layernorm_forward(x, gamma, beta, residual=None, eps=1e-5, out_dtype=None, c
         ldr = _train_rows(name, "residual", residual, C)[1]
     _train_vec(name, "gamma", gamma, C)
     _train_vec(name, "beta", beta, C)
-    y = torch.empty(x.shape, dtype=x.dtype if out_dtype is None else out_dtype, device=x.device)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else x
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    y = _like(x, x.dtype if out_dtype is None else out_dtype)
+    total = _like(x, x.dtype) if residual is not None else x
+    stats = gamma.new_empty((rows, 2))
     ck = _new_ckpt(rows, C, x.device) if checkpoint else None
     if rows:
         _lib.run("ovis_layernorm_train_forward", "plplppppppplifiip", x.data_ptr(), ldx, _ptr(residual), ldr, gamma.data_ptr(), beta.data_ptr(),
@@ -1182,10 +1187,10 @@ def layernorm_backward(dy, x, stats, gamma, dsum=None, out_dtype=None):
     if stats.dtype != torch.float32 or stats.numel() != 2 * rows or not stats.is_contiguous():
         raise _lib.OvisError(f"{name}: stats must be contiguous float32 [{rows}, 2]")
     _train_vec(name, "gamma", gamma, C)
-    dx = torch.empty(dy.shape, dtype=xdt, device=dy.device)
+    dx = _like(dy, xdt)
     if not rows:
         return dx, torch.zeros((C,), dtype=torch.float32, device=dy.device), torch.zeros((C,), dtype=torch.float32, device=dy.device)
-    grads = torch.empty((2, C), dtype=torch.float32, device=dy.device)
+    grads = gamma.new_empty((2, C))
     ws = _workspace("ovis_layernorm_train_backward_workspace_bytes", "lii", dy.device, rows, C, xd)
     dgamma, dbeta = grads.unbind(0)
     _lib.run("ovis_layernorm_train_backward", "plplppppplppppliiip", dy.data_ptr(), lddy, x.data_ptr() if ck is None else None, ldx,
@@ -1224,7 +1229,7 @@ def _act_ckpt8(name, h, act):
     _train_check(name, h)
     d = _train_dtype(name, "input", h)
     rows, ldh = _train_rows(name, "input", h, C)
-    y = torch.empty(h.shape, dtype=h.dtype, device=h.device) if act else None
+    y = _like(h, h.dtype) if act else None
     ck = _new_ckpt(rows, C, h.device)
     if rows:
         _lib.run("ovis_act_ckpt8_forward", "plpppliiip", h.data_ptr(), ldh, _ptr(y), ck.codes.data_ptr(), ck.scales.data_ptr(), rows, C, int(act), d,
@@ -1244,7 +1249,7 @@ def act_backward_ckpt8(dy, h8, act, recompute=False):
     drows, lddy = _train_rows(name, "dy", dy, C)
     if drows != rows:
         raise _lib.OvisError(f"{name}: dy has {drows} rows, the 8-bit rows are {rows}")
-    dh = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dh = _like(dy, dy.dtype)
     y8 = _new_ckpt(rows, C, dy.device) if recompute else None
     if not rows:
         return dh, torch.zeros((C,), dtype=torch.float32, device=dy.device), y8
@@ -1306,7 +1311,7 @@ def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset
     row = (Nk + v - 1) // v * v if ld is None else int(ld)
     if row < Nk or row % v:
         raise _lib.OvisError(f"{name}: ld must be at least {Nk} and a multiple of {v}")
-    out = torch.empty((H, Nq, row), dtype=out_dtype, device=table.device)
+    out = table.new_empty((H, Nq, row), dtype=out_dtype)
     if Nq and Nk:
         _lib.run("ovis_relpos_bias_1d", "pppiiiiiilip", table.data_ptr(), out.data_ptr(), borders, nb, int(bool(bidirectional)), H, Nq, Nk, row, off, d,
                  _lib.raw_stream())

@@ -110,8 +110,9 @@ act_ckpt8_bwd_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __
   unsigned sn;
   auto fetch = [&](long long r) {
     const int m = r < r1 ? n : 0;
-    dn.load(dy + r * lddy + col, m);
-    qn = load_codes(codes + r * C + col, m);
+    const bool on = r + 8 < rows;                                // eight rows on, a row's end is not the tensor's
+    dn.load(dy + r * lddy + col, m, on);
+    qn = load_codes(codes + r * C + col, m, on);
     sn = m > 0 ? scales[r * nblk + (col >> 5)] : 127u;
   };
   fetch(r0 + ri);
@@ -123,7 +124,7 @@ act_ckpt8_bwd_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __
     const unsigned sb0 = sn;
     if (rb + rp < r1) fetch(r + rp);
     float h[8], d[8];
-    decode8(q, sb0, h);
+    decode8(q, sb0, h);                                          // behind the row's end: values that are neither stored nor summed up
 #pragma unroll
     for (int e = 0; e < 8; ++e) d[e] = raw.at(e);
 #pragma unroll
@@ -183,6 +184,7 @@ inline BwdShape bwd_shape(long long rows, int C) {
   const long long most = (rows + rp - 1) / rp;                   // at least one pass of rows a workgroup
   long long want = s.strips < 1536 ? 1536 / s.strips : 1;        // six workgroups a CU in all: what is there at once
   if (want > most) want = most;
+  if (most <= 4) want = 1;                                       // and no second launch: the workgroup's sums are the gradient
   s.chunk = ((rows + want - 1) / want + rp - 1) / rp * rp;
   s.chunks = (unsigned)((rows + s.chunk - 1) / s.chunk);
   return s;
@@ -226,15 +228,16 @@ extern "C" int ovis_act_ckpt8_backward(const void* dy, long long lddy, const uin
   OVIS_REQUIRE(rows > 0 && C > 0 && C <= (1 << 30) && lddy >= C, "act_ckpt8_backward: rows %lld, columns %d, row stride %lld", rows, C, lddy);
   const BwdShape s = bwd_shape(rows, C);
   OVIS_REQUIRE(s.chunks <= 65535, "act_ckpt8_backward: too many rows for one launch");
+  float* to = s.chunks == 1 ? dbias : workspace;
 #define ACT_GO(T, A)                                                                                                                        \
   hipLaunchKernelGGL((act_ckpt8_bwd_kernel<T, A>), dim3(s.strips, s.chunks), dim3(256), 0, (hipStream_t)stream, (const T*)dy, lddy, codes, \
-                     scales, (T*)dh, codes_out, scales_out, workspace, rows, s.chunk, s.lshift, C)
+                     scales, (T*)dh, codes_out, scales_out, to, rows, s.chunk, s.lshift, C)
 #define ACT_ALL(T) switch (act) { case 1: ACT_GO(T, 1); break; case 2: ACT_GO(T, 2); break; default: ACT_GO(T, 3); }
   ACT_TYPE(dtype, ACT_ALL)
 #undef ACT_GO
 #undef ACT_ALL
   const int rc = ovis::check_launch("act_ckpt8_backward");
-  if (rc != OVIS_OK) return rc;
+  if (rc != OVIS_OK || s.chunks == 1) return rc;
   return ovis::column_sum_finish(workspace, (int)s.chunks, C, dbias, C, dbias, (hipStream_t)stream);
 }
 

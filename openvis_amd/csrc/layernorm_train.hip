@@ -102,11 +102,12 @@ layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __
   }
 }
 
-// TX: x, dsum and dx; TY: dy; CK: the normalised rows come in 8 bits.  A workgroup walks over rows and keeps dgamma / dbeta of its lanes' columns
+// TX: x, dsum and dx; TY: dy; CK: the normalised rows come in 8 bits; TAIL: C is no multiple of 8, a row's last piece is masked (a variant of its
+// own: a mask in the other costs it the fetch ahead, 109 -> 144 us).  A workgroup walks over rows and keeps dgamma / dbeta of its lanes' columns
 // in registers, gamma in LDS.  The next row is fetched before the present one's sums begin, and rows stay in their stored width until they are
 // used: the sums take two dependent passes over a row, in which a wavefront without the next row's loads would have nothing in flight.
 // 98500 x 768 fp16 from 8 bits with dsum: 109 us, 4.9 TB/s (without the fetch ahead 133 us; a large copy reaches 5.0 TB/s).
-template <typename TX, typename TY, bool CK, int LPR, int NCH, int WAVES>
+template <typename TX, typename TY, bool CK, bool TAIL, int LPR, int NCH, int WAVES>
 __global__ void __launch_bounds__(256, WAVES)
 layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
                            const uint8_t* __restrict__ scales, const float* __restrict__ stats, const float* __restrict__ gamma,
@@ -129,17 +130,19 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
   unsigned qsn[NCH];
   float meann, rstdn;
   auto fetch = [&](long long row) {
-    const bool live = row < rows;
+    const bool live = row < rows, on = row + 8 < rows;           // eight rows on, a row's end is not the tensor's
     const long long r = live ? row : rows - 1;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = (c * LPR + li) * 8, n = live ? C - col : 0;
-      dn[c].load(dy + r * lddy + col, n);
+      if constexpr (TAIL) dn[c].load(dy + r * lddy + col, n, on);
+      else dn[c].load_all(dy + r * lddy + col, n > 0);
       if constexpr (CK) {
-        qn[c] = load_codes(codes + r * C + col, n);
+        qn[c] = TAIL ? load_codes(codes + r * C + col, n, on) : load_codes(codes + r * C + col, n > 0 ? 8 : 0);
         qsn[c] = n > 0 ? scales[r * nblk + (col >> 5)] : 127u;
       } else {
-        hn[c].load(x + r * ldx + col, n);
+        if constexpr (TAIL) hn[c].load(x + r * ldx + col, n, on);
+        else hn[c].load_all(x + r * ldx + col, n > 0);
       }
     }
     meann = stats[2 * r], rstdn = stats[2 * r + 1];
@@ -147,7 +150,8 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
         const int col = (c * LPR + li) * 8;
-        tn[c].load(dsum + r * ldds + col, live ? C - col : 0);
+        if constexpr (TAIL) tn[c].load(dsum + r * ldds + col, live ? C - col : 0, on);
+        else tn[c].load_all(dsum + r * ldds + col, live && C > col);
       }
   };
   int phase = 0;
@@ -177,11 +181,13 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const float* g = acc + (c * LPR + li) * 8;
+      const int n = C - (c * LPR + li) * 8;
       float v[8];
       xhat(c, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float de = d[c].at(e), gd = de * g[e];
+        if constexpr (TAIL && CK) v[e] = e < n ? v[e] : 0.f;     // without codes xhat has done so
+        const float de = TAIL && e >= n ? 0.f : d[c].at(e), gd = de * g[e];
         s1 += gd;
         s2 += gd * v[e];
         dg[c][e] += de * v[e];
@@ -251,7 +257,9 @@ inline RowShape bwd_row_shape(int C, int x_dtype) { return row_shape(C, x_dtype 
 // as many workgroups as the card holds at once: each walks over its rows, and a workgroup that had to wait would walk alone at the end
 constexpr int bwd_waves(int nch) { return nch == 1 ? 4 : 2; }
 inline unsigned bwd_blocks(long long rows, const RowShape& s) {
-  const long long need = (rows + 256 / s.lpr - 1) / (256 / s.lpr), most = 256 * bwd_waves(s.nch);
+  const long long need = (rows + 256 / s.lpr - 1) / (256 / s.lpr), full = 256 * bwd_waves(s.nch);
+  if (need <= 4) return 1;                                       // and no second launch: the workgroup's sums are the gradients
+  const long long most = rows / 10 < 256 ? 256 : rows / 10 < full ? rows / 10 : full;    // a workgroup's line of sums costs as much as three rows
   return (unsigned)(need < most ? need : most);
 }
 
@@ -261,8 +269,8 @@ namespace ovis {
 
 // out0[w] (w < split), out1[w - split] = sum over the P lines of part [P][W], in a fixed order.  Two forms:
 // narrow: 64 lanes of a column take every 64th line, then a tree; 16 columns a workgroup, so that the lines, which come from L2, are read by
-// many workgroups.  wide: a lane takes four columns and all lines.  The wide form needs no exchange but fills the card only from some
-// thousands of columns on: 33 lines of 124416 columns 5 us against 20, 1024 lines of 1536 columns 60 us against 5.
+// many workgroups.  wide: a lane takes four columns and all lines.  The wide form needs no exchange but fills the card only from
+// tens of thousands of columns on: 33 lines of 124416 columns 5 us against 20, 126 lines of 29282 columns 40 us against 6.
 __global__ void __launch_bounds__(1024)
 column_sum_narrow_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
   __shared__ float buf[64][17];
@@ -313,7 +321,7 @@ column_sum_wide_kernel(const float* __restrict__ part, int P, int W, float* __re
 }
 
 int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream) {
-  if (W >= 128 * P && W >= 16384)
+  if (W >= 65536)
     hipLaunchKernelGGL(column_sum_wide_kernel, dim3(cdiv(W, 1024)), dim3(256), 0, stream, part, P, W, out0, split, out1);
   else
     hipLaunchKernelGGL(column_sum_narrow_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, part, P, W, out0, split, out1);
@@ -382,17 +390,20 @@ extern "C" int ovis_layernorm_train_backward(const void* dy, long long lddy, con
                "layernorm_train_backward: dy has x's type, or any where x is f32");
   const RowShape sh = bwd_row_shape(C, x_dtype);
   const unsigned blocks = bwd_blocks(rows, sh);
+  float* to = blocks == 1 && dbeta == dgamma + C ? dgamma : workspace;
 #define LN_GO(TX, TY, LPR, NCH)                                                                                                             \
-  if (codes) LN_RUN(TX, TY, true, LPR, NCH);                                                                                                \
-  else LN_RUN(TX, TY, false, LPR, NCH)
-#define LN_RUN(TX, TY, CK, LPR, NCH)                                                                                                        \
-  hipLaunchKernelGGL((layernorm_train_bwd_kernel<TX, TY, CK, LPR, NCH, bwd_waves(NCH)>), dim3(blocks),          \
+  if (codes && C % 8) LN_RUN(TX, TY, true, true, LPR, NCH);                                                                                 \
+  else if (codes) LN_RUN(TX, TY, true, false, LPR, NCH);                                                                                    \
+  else if (C % 8) LN_RUN(TX, TY, false, true, LPR, NCH);                                                                                    \
+  else LN_RUN(TX, TY, false, false, LPR, NCH)
+#define LN_RUN(TX, TY, CK, TAIL, LPR, NCH)                                                                                                  \
+  hipLaunchKernelGGL((layernorm_train_bwd_kernel<TX, TY, CK, TAIL, LPR, NCH, bwd_waves(NCH)>), dim3(blocks),                                \
                      dim3(256), 2 * LPR * NCH * 8 * 4, (hipStream_t)stream, (const TY*)dy, lddy, (const TX*)x, ldx, codes, scales, stats,   \
-                     gamma, (const TX*)dsum, ldds, (TX*)dx, workspace, rows, C)
+                     gamma, (const TX*)dsum, ldds, (TX*)dx, to, rows, C)
   LN_TYPES(x_dtype, dy_dtype, LN_MOST2, LN_MOST3)
 #undef LN_GO
 #undef LN_RUN
   const int rc = ovis::check_launch("layernorm_train_backward");
-  if (rc != OVIS_OK) return rc;
+  if (rc != OVIS_OK || to != workspace) return rc;
   return ovis::column_sum_finish(workspace, (int)blocks, 2 * C, dgamma, C, dbeta, (hipStream_t)stream);
 }

@@ -69,36 +69,38 @@ relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders 
 
 // Diagonal sums.  A wavefront owns 64 V diagonals, V neighbouring ones a lane, and walks down the rows of its share: the lane's V elements
 // of the next row lie one element on, so they are loaded as one vector at any element's address and added to the same registers -- no
-// transposition, no LDS, no atomics.  A vector that crosses an end of its row is read all the same, from the neighbouring rows' elements, and
+// transposition, no LDS, no atomics.  Where a row is short, L < 64 lanes take 8 L diagonals and 64 / L rows go at once: a strip of 8 L diagonals
+// meets rows of Nk columns, so 8 L beyond Nk is idle (9 x 20 x 3834 x 32 f32: 102 us with 64 lanes).  A vector that crosses an end of its row is read all the same, from the neighbouring rows' elements, and
 // masked; only where it would leave the tensor's span (first and last rows) are its elements read one by one: a separate read of a row's ends
 // cost more than the rows themselves (8 x 8 x 1023^2 bf16: 50 us).  A workgroup is four wavefronts on the same diagonals, rows dealt in turn;
 // its sums are one line of the workspace.  grid: (diagonal strips, row chunks x batch, heads).
-template <typename T>
+template <typename T, int L>
 __global__ void __launch_bounds__(256)
 relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, long long B, int bper, int Nq,
                   int Nk, int rows, int chunks) {
-  constexpr int V = 8, U = 4;                                    // U rows in flight
-  __shared__ float buf[4][64 * V + 4];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int V = 8, U = 4, RG = 256 / L;                      // U rows in flight, RG row groups
+  __shared__ float buf[RG][L * V + 4];
+  const int lane = threadIdx.x % L;
+  const int grp = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / L;
   const int h = blockIdx.z, ck = blockIdx.y % chunks;
   const long long b0 = (long long)(blockIdx.y / chunks) * bper, b1 = b0 + bper < B ? b0 + bper : B;
   const long long span = (B - 1) * bs + (long long)(gridDim.z - 1) * hs + (long long)(Nq - 1) * ld + Nk;
   const int D = Nq + Nk - 1;
-  const int d0 = blockIdx.x * 64 * V;                            // diagonal index d: j = i + d - (Nq - 1)
+  const int d0 = blockIdx.x * L * V;                             // diagonal index d: j = i + d - (Nq - 1)
   const int dl = d0 + lane * V - (Nq - 1);
   // rows that meet this strip: 0 <= i + d - (Nq - 1) < Nk for some d of it
-  const int lo = max(max(ck * rows, Nq - 1 - (d0 + 64 * V - 1)), 0), hi = min(min((ck + 1) * rows, Nq), Nk + Nq - 1 - d0);
+  const int lo = max(max(ck * rows, Nq - 1 - (d0 + L * V - 1)), 0), hi = min(min((ck + 1) * rows, Nq), Nk + Nq - 1 - d0);
   float acc[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) acc[e] = 0.f;
   for (long long b = b0; b < b1; ++b) {
     const long long at = b * bs + (long long)h * hs;
-    for (int i = lo + wave; i < hi; i += 4 * U) {
+    for (int i = lo + grp; i < hi; i += RG * U) {
       Raw8<T> v[U];
-      const bool inside = i + d0 - (Nq - 1) >= 0 && i + 4 * (U - 1) + d0 - (Nq - 1) + 64 * V <= Nk && i + 4 * (U - 1) < hi;
+      const bool inside = i + d0 - (Nq - 1) >= 0 && i + RG * (U - 1) + d0 - (Nq - 1) + L * V <= Nk && i + RG * (U - 1) < hi;
       if (inside) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load_all(g + at + (i + 4 * u) * ld + (i + 4 * u + dl), true);
+        for (int u = 0; u < U; ++u) v[u].load_all(g + at + (i + RG * u) * ld + (i + RG * u + dl), true);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -107,7 +109,7 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
         bool alone[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int r = i + 4 * u, j = r + dl;
+          const int r = i + RG * u, j = r + dl;
           const long long o = at + r * ld + j;
           const bool any = r < hi && j > -V && j < Nk;
           alone[u] = any && (o < 0 || o + V > span);
@@ -115,14 +117,14 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int j = i + 4 * u + dl;
+          const int j = i + RG * u + dl;
 #pragma unroll
           for (int e = 0; e < V; ++e) acc[e] += (unsigned)(j + e) < (unsigned)Nk ? v[u].at(e) : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (alone[u]) {
-            const int r = i + 4 * u, j = r + dl;
+            const int r = i + RG * u, j = r + dl;
             const T* p = g + at + r * ld + j;
 #pragma unroll
             for (int e = 0; e < V; ++e)
@@ -133,11 +135,16 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
     }
   }
 #pragma unroll
-  for (int e = 0; e < V; ++e) buf[wave][lane * V + e] = acc[e];
+  for (int e = 0; e < V; ++e) buf[grp][lane * V + e] = acc[e];
   __syncthreads();
   float* line = part + ((long long)blockIdx.y * gridDim.z + h) * D;
-  for (int k = threadIdx.x; k < 64 * V; k += 256)
-    if (d0 + k < D) line[d0 + k] = (buf[0][k] + buf[1][k]) + (buf[2][k] + buf[3][k]);
+  for (int k = threadIdx.x; k < L * V; k += 256)
+    if (d0 + k < D) {
+      float t = buf[0][k];
+#pragma unroll
+      for (int w = 1; w < RG; ++w) t += buf[w][k];
+      line[d0 + k] = t;
+    }
 }
 
 // sum over a workgroup's 256 values, in a fixed order
@@ -176,6 +183,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, int H, int N, int nvec,
                        long long B, long long chunk) {
+  const long long span = (B - 1) * bs + (long long)(H - 1) * hs + (long long)(N - 1) * ld + N;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long long)H * N * nvec) return;
   const int v = (int)(i % nvec);
@@ -186,8 +194,21 @@ window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  // what a row's last lane reads beyond it lies in the tensor up to the last batch entries, and is not stored
+  const long long here = (long long)h * hs + (long long)row * ld + v * 8;
+  long long bv = b1;
+  if (n < 8) {
+    while (bv > b0 && here + (bv - 1) * bs + 8 > span) --bv;     // a step or two, or all where the batch is one entry broadcast
+  }
+  long long b = b0;
 #pragma unroll 4
-  for (long long b = b0; b < b1; ++b) {
+  for (; b < bv; ++b) {
+    Raw8<T> x;
+    x.load_all(p + b * bs, true);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += x.at(e);
+  }
+  for (; b < b1; ++b) {
     float x[8];
     load8(p + b * bs, n, x);
 #pragma unroll
@@ -196,29 +217,37 @@ window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long
   store8(part + (((long long)blockIdx.y * H + h) * N + row) * N + v * 8, n, acc);
 }
 
+// A workgroup takes the pairs of one vertical offset and head: a lane the pairs (xi, xj), whose rows of ws elements it adds over the token rows
+// yj, then one of the 2 ws - 1 horizontal offsets each.
 __global__ void __launch_bounds__(256)
 window_bias_finish_kernel(const float* __restrict__ sum, float* __restrict__ dtable, int H, int ws) {
-  __shared__ float buf[256];
-  const int bk = blockIdx.x, h = blockIdx.y, N = ws * ws, w = 2 * ws - 1;
-  const int dy = bk / w - (ws - 1), dx = bk % w - (ws - 1);      // yi - yj, xi - xj
-  const int ny = ws - abs(dy), nx = ws - abs(dx), n = ny * nx;
-  float s = 0.f;
-  for (int t = threadIdx.x; t < n; t += 256) {
-    const int yj = max(0, -dy) + t / nx, xj = max(0, -dx) + t % nx;
-    s += sum[((long long)h * N + (yj + dy) * ws + xj + dx) * N + yj * ws + xj];
+  extern __shared__ float pair[];                                // [xi][xj]
+  const int h = blockIdx.y, N = ws * ws, w = 2 * ws - 1, dy = (int)blockIdx.x - (ws - 1);          // yi - yj
+  const int y0 = max(0, -dy), y1 = min(ws, ws - dy);             // yj
+  for (int t = threadIdx.x; t < N; t += 256) {
+    const int xi = t / ws, xj = t - xi * ws;
+    float s = 0.f;
+    for (int yj = y0; yj < y1; ++yj) s += sum[((long long)h * N + (yj + dy) * ws + xi) * N + yj * ws + xj];
+    pair[t] = s;
   }
-  s = block_sum(s, buf);
-  if (threadIdx.x == 0) dtable[(long long)bk * H + h] = s;
+  __syncthreads();
+  for (int k = threadIdx.x; k < w; k += 256) {
+    const int dx = k - (ws - 1), x0 = max(0, -dx), x1 = min(ws, ws - dx);
+    float s = 0.f;
+    for (int xj = x0; xj < x1; ++xj) s += pair[(xj + dx) * ws + xj];
+    dtable[((long long)blockIdx.x * w + k) * H + h] = s;
+  }
 }
 
-// Workgroups: about sixteen a CU; a long sequence's rows are split (32 at least a workgroup), a large batch's entries go several to one.
-struct SeqShape { int strips, chunks, rows, bper; long long lines; };
+// Workgroups: about sixteen a CU; a long sequence's rows are split, a large batch's entries go several to one.
+struct SeqShape { int lanes, strips, chunks, rows, bper; long long lines; };
 inline SeqShape seq_shape(long long B, int H, int Nq, int Nk) {
   SeqShape s;
-  s.strips = (int)(((long long)Nq + Nk - 1 + 511) / 512);
+  s.lanes = Nk >= 512 ? 64 : Nk >= 256 ? 32 : Nk >= 128 ? 16 : 8;
+  s.strips = (int)(((long long)Nq + Nk - 1 + 8 * s.lanes - 1) / (8 * s.lanes));
   const long long per = B * H * s.strips;
   long long want = (4096 + per - 1) / per;
-  const long long most = (Nq + 31) / 32;
+  const long long most = (Nq + 2048 / s.lanes - 1) / (2048 / s.lanes);              // eight passes of rows at least
   if (want > most) want = most;
   s.rows = (int)((Nq + want - 1) / want);
   s.chunks = (Nq + s.rows - 1) / s.rows;
@@ -297,10 +326,13 @@ extern "C" int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, lon
   const SeqShape s = seq_shape(B, H, Nq, Nk);
   const long long W = (long long)H * (Nq + Nk - 1);
   OVIS_REQUIRE(s.lines <= 65535 && W < (1ll << 31), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
-#define RP_GO(T)                                                                                                                            \
-  hipLaunchKernelGGL((relpos_bwd_kernel<T>), dim3(s.strips, (unsigned)s.lines, H), dim3(256), 0, (hipStream_t)stream, (const T*)dbias, bs,  \
+#define RP_LANES(T)                                                                                                                         \
+  if (s.lanes == 64) { RP_GO(T, 64) } else if (s.lanes == 32) { RP_GO(T, 32) } else if (s.lanes == 16) { RP_GO(T, 16) } else { RP_GO(T, 8) }
+#define RP_GO(T, L)                                                                                                                         \
+  hipLaunchKernelGGL((relpos_bwd_kernel<T, L>), dim3(s.strips, (unsigned)s.lines, H), dim3(256), 0, (hipStream_t)stream, (const T*)dbias, bs,  \
                      hs, ld, workspace + W, B, s.bper, Nq, Nk, s.rows, s.chunks);
-  RP_TYPE(dtype, RP_GO)
+  RP_TYPE(dtype, RP_LANES)
+#undef RP_LANES
 #undef RP_GO
   int rc2 = ovis::check_launch("relpos_bias_1d_backward");
   if (rc2 == OVIS_OK && s.lines > 1)
@@ -335,7 +367,7 @@ extern "C" int ovis_swin_relpos_bias_backward(const void* dbias, long long bs, l
   if (rc == OVIS_OK && s.chunks > 1)
     rc = ovis::column_sum_finish(workspace + W, s.chunks, (int)W, workspace, (int)W, workspace, (hipStream_t)stream);
   if (rc != OVIS_OK) return rc;
-  hipLaunchKernelGGL(window_bias_finish_kernel, dim3((2 * ws - 1) * (2 * ws - 1), H), dim3(256), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(window_bias_finish_kernel, dim3(2 * ws - 1, H), dim3(256), N * 4, (hipStream_t)stream,
                      s.chunks > 1 ? workspace : workspace + W, dtable, H, ws);
   return ovis::check_launch("swin_relpos_bias_backward");
 }

@@ -39,12 +39,18 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)
 template <typename T>
 struct Raw8 {
   typename Vec8Of<T>::type v;
-  __device__ __forceinline__ void load(const T* __restrict__ p, int n) {
-    if (n >= 8) {
-      v = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
-    } else {
+  // n elements of a row at p, the others anything (n <= 0: 0).  on: the eight lie in the tensor even where the row ends earlier (the next rows
+  // follow): they are read as one vector, which nothing waits for
+  __device__ __forceinline__ void load(const T* __restrict__ p, int n, bool on) {
+    v = (typename Vec8Of<T>::type)0;
+    if (n > 0) {
+      if (n >= 8 || on) {
+        v = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? p[e] : (T)0.f;
+        for (int e = 0; e < 7; ++e)
+          if (e < n) v[e] = p[e];
+      }
     }
   }
   __device__ __forceinline__ void load_all(const T* __restrict__ p, bool any) {       // all eight, or none
@@ -155,6 +161,9 @@ __device__ __forceinline__ u32x2_u load_codes(const uint8_t* __restrict__ p, int
   }
   return c;
 }
+
+// the same, with the codes behind the row's end where `on` says that they can be read
+__device__ __forceinline__ u32x2_u load_codes(const uint8_t* __restrict__ p, int n, bool on) { return load_codes(p, n > 0 && on ? 8 : n); }
 
 __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int n, u32x2_u c) {
   if (n >= 8) {

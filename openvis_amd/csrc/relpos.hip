@@ -299,7 +299,7 @@ extern "C" int ovis_relpos_bias_1d(const float* table, void* out, const int* bor
   const unsigned strips = ovis::cdiv(ld, cols);
   int rows = 64;
   while ((long long)((Nq + rows - 1) / rows) > 65535) rows *= 2;
-  OVIS_REQUIRE(rows <= 16384, "relpos_bias_1d: too many rows");
+  OVIS_REQUIRE(rows <= 8192, "relpos_bias_1d: too many rows");
 #define RP_GO(T)                                                                                                                            \
   hipLaunchKernelGGL((relpos_fwd_kernel<T>), dim3(strips, (Nq + rows - 1) / rows, H), dim3(256), (cols + rows) * sizeof(T),                 \
                      (hipStream_t)stream, table, (T*)out, b, bidirectional, H, Nq, Nk, ld, q_offset, rows);

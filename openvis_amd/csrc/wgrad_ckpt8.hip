@@ -111,7 +111,7 @@ __device__ __forceinline__ u16x8 widen(u32x2_u c, float f) {
 template <typename T, int TN, int TK, int WN, int WK, int BM>
 __global__ void __launch_bounds__(64 * WN * WK)
 wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                   float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k) {
+                   float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k, int turns) {
   constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
   constexpr int P = sizeof(T) == 4 ? 3 : 1, NT = 64 * WN * WK, RN = TN / WN, RK = TK / WK, AN = RN / 32, AK = RK / 32, NS = BM / 16;
   constexpr int YR = NT / (TN / 8), XR = NT / (TK / 8), YP = BM / YR, XP = BM / XR;        // rows a pass, passes
@@ -195,8 +195,8 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   float dsum[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) dsum[e] = 0.f;
-  // db: every workgroup of these rows and columns n stages all of dY; they take the steps in turn
-  int turn = kt;
+  // db: every workgroup of these rows and columns n stages all of dY; the first `turns` of them take the steps in turn
+  int turn = kt < turns ? kt : -1;
   auto sum_rows = [&](const Rows& R, bool valid) {
     if (turn == 0 && valid) {
 #pragma unroll
@@ -204,7 +204,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
 #pragma unroll
         for (int e = 0; e < 8; ++e) dsum[e] += R.y[i].value(e);
     }
-    turn = turn == 0 ? tiles_k - 1 : turn - 1;
+    turn = turn == 0 ? turns - 1 : turn < 0 ? -1 : turn - 1;
   };
   auto stage_piece = [&](const Rows& R, int buf, int i) {
     if (i < YP) {
@@ -326,7 +326,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       if (t + 4 < nf) step(t + 4, I1{}, I0{});
     }
   }
-  turn = (int)((kt - nf % tiles_k + tiles_k) % tiles_k);         // the steps of the loop were counted beyond its end
+  if (kt < turns) turn = (int)((kt - nf % turns + turns) % turns);               // the steps of the loop were counted beyond its end
   for (long long m = m0 + nf * BM; m < m1; m += BM) {
     Rows R;
     fetch_masked(R, m);
@@ -361,6 +361,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
         }
     }
   }
+  if (kt >= turns) return;
   float* sum = reinterpret_cast<float*>(lds);                    // db: the lanes of a column group, in order: [YR][TN]
 #pragma unroll
   for (int e = 0; e < 8; ++e) sum[yr * TN + yc + e] = dsum[e];
@@ -368,7 +369,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   for (int c = tid; c < TN; c += NT) {
     float t = 0.f;
     for (int i = 0; i < YR; ++i) t += sum[i * TN + c];
-    if (n0 + c < N) dbp[(s * tiles_k + kt) * N + n0 + c] = t;
+    if (n0 + c < N) dbp[(s * turns + kt) * N + n0 + c] = t;
   }
 }
 
@@ -406,7 +407,7 @@ wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict
   }
 }
 
-struct WgradShape { int tile, tiles_n, tiles_k, S; long long chunk; };
+struct WgradShape { int tile, tiles_n, tiles_k, S; long long chunk; int turns; };
 // Tile and split by a model of the time (us), fitted to sweeps over shapes of 100 to 294400 rows and 8 to 4096 columns:
 //   a step of 32 rows takes `one` where a CU has one workgroup, and `more` longer for each further one, up to `most` at once; then they go in
 //   rounds.  16-bit: tile 256 1.0; 128 0.45 and 0.23; 64 0.43 and 0.22.  f32 (three products): 128 0.98 and 0.58; 64 0.45 and 0.25;
@@ -434,7 +435,8 @@ inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
       const double t = rounds * (chunk / 32) * (one + more * (per - 1)) + (parts > 1 ? 3.0 + 8.0 * parts * N * K / 4.5e6 : 0.0);
       if (t < least) {
         least = t;
-        best = {tile, (int)tn, (int)tk, (int)parts, chunk};
+        // one part of a few steps: one workgroup sums dY for db, and no second launch adds up what several would have
+        best = {tile, (int)tn, (int)tk, (int)parts, chunk, parts == 1 && chunk <= 512 ? 1 : (int)tk};
       }
     }
   }
@@ -446,7 +448,7 @@ inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
 extern "C" long long ovis_linear_wgrad_ckpt8_workspace_bytes(long long M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || !ovis::dtype_ok(dtype)) return 0;
   const WgradShape w = wgrad_shape(M, N, K, dtype);
-  return ((long long)w.S * N * K + (long long)w.S * w.tiles_k * N + ((long long)N * K < 65536 ? (long long)N * K : 0)) * 4;
+  return ((long long)w.S * N * K + (long long)w.S * w.turns * N + ((long long)N * K < 65536 ? (long long)N * K : 0)) * 4;
 }
 
 extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, const float* gamma,
@@ -461,16 +463,18 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
                K, lddy);
   const bool join = w.S > 1 || gamma;
   float* part = join ? workspace : dw;
-  const int lines = w.S * w.tiles_k;
+  const int lines = w.S * w.turns;
   float* dbp = lines > 1 ? workspace + (long long)w.S * N * K : db;
 #define WG_GO(T, TN, TK, WN, WK, BM)                                                                                                        \
   {                                                                                                                                         \
     const int lds = 3 * BM * (TN * (sizeof(T) == 4 ? 3 : 1) + TK) * 2;                                                                      \
-    const hipError_t e = hipFuncSetAttribute((const void*)wgrad_ckpt8_kernel<T, TN, TK, WN, WK, BM>,                                        \
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                              \
-    OVIS_REQUIRE(e == hipSuccess, "linear_wgrad_ckpt8: %s", hipGetErrorString(e));                                                          \
+    if (lds > 65536) {                                                                                                                      \
+      const hipError_t e = hipFuncSetAttribute((const void*)wgrad_ckpt8_kernel<T, TN, TK, WN, WK, BM>,                                      \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);                                            \
+      if (e != hipSuccess) return ovis::fail(OVIS_ELAUNCH, "linear_wgrad_ckpt8: %s", hipGetErrorString(e));                                 \
+    }                                                                                                                                       \
     hipLaunchKernelGGL((wgrad_ckpt8_kernel<T, TN, TK, WN, WK, BM>), dim3((unsigned)blocks), dim3(64 * WN * WK), lds, (hipStream_t)stream,   \
-                       (const T*)dy, lddy, codes, scales, part, dbp, M, N, K, w.chunk, w.tiles_n, w.tiles_k);                               \
+                       (const T*)dy, lddy, codes, scales, part, dbp, M, N, K, w.chunk, w.tiles_n, w.tiles_k, w.turns);                      \
   }
   if (dtype == OVIS_F32) {
     if (w.tile == 128) WG_GO(float, 128, 128, 2, 2, 16)

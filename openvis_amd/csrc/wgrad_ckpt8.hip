@@ -43,11 +43,12 @@ __device__ __forceinline__ f32x16 mfma(u16x8 a, u16x8 b, f32x16 c) {
 }
 
 // an LDS tile [rows][W] of 16-bit elements; the 32-column pieces of a row are permuted by the row, so that the four rows of a transposing
-// read lie in different banks
+// read lie in different banks, and of 256 columns the upper ones have the halves of a piece exchanged, so that eight lanes that write a
+// piece each (X's codes) do too
 template <int W>
 __device__ __forceinline__ int at(int m, int c) {
-  const int s = W >= 128 ? m & 3 : (m >> 1) & 1;
-  return m * W + ((((c >> 5) ^ s) << 5) | (c & 31));
+  const int s = W >= 128 ? m & 3 : (m >> 1) & 1, x = W == 256 ? (c >> 3) & 16 : 0;
+  return m * W + ((((c >> 5) ^ s) << 5) | ((c & 31) ^ x));
 }
 
 template <typename T> struct DyOf {                              // 8 elements of dY as loaded
@@ -114,8 +115,9 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
                    float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k, int turns) {
   constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
   constexpr int P = sizeof(T) == 4 ? 3 : 1, NT = 64 * WN * WK, RN = TN / WN, RK = TK / WK, AN = RN / 32, AK = RK / 32, NS = BM / 16;
-  constexpr int YR = NT / (TN / 8), XR = NT / (TK / 8), YP = BM / YR, XP = BM / XR;        // rows a pass, passes
-  static_assert(YP * YR == BM && XP * XR == BM && YP > 0 && XP > 0, "a step is whole passes");
+  constexpr int YR = NT / (TN / 8), YP = BM / YR;                // dY: rows a pass, passes of eight columns a lane
+  constexpr int XC = BM * TK / NT, XP = XC / 8;                  // X: columns a lane takes of one row, inside one block of 32: one scale
+  static_assert(YP * YR == BM && YP > 0 && XC * NT == BM * TK && (XC == 8 || XC == 16 || XC == 32), "a step is whole passes");
   extern __shared__ unsigned short lds[];
   unsigned short* const ly = lds;                                // [3][P][BM][TN]
   unsigned short* const lx = lds + 3 * P * BM * TN;              // [3][BM][TK]
@@ -161,21 +163,30 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
     __syncthreads();
   }
 
-  const int yr = tid / (TN / 8), yc = (tid % (TN / 8)) * 8, xr = tid / (TK / 8), xc = (tid % (TK / 8)) * 8;
+  const int yr = tid / (TN / 8), yc = (tid % (TN / 8)) * 8, xr = tid / (TK / XC), xc = (tid % (TK / XC)) * XC;
   const int yn = N - n0 - yc, xn = K - k0 - xc;                  // columns from this lane's first on
   const int xtop = F16 ? top[xc >> 5] - 7 : 0;
-  struct Rows { DyOf<T> y[YP]; u32x2_u x[XP]; unsigned s[XP]; };
+  struct Rows { DyOf<T> y[YP]; u32x2_u x[XP]; unsigned s; };
   // no masks; a step's uniform row pointers and a lane's 32-bit offsets from them; in pieces, to lie between the products
   struct At { const T* y; const uint8_t *c, *s; };
   const unsigned oy = yr * (unsigned)lddy + (yn > 0 ? n0 + yc : 0), oc = xr * (unsigned)K + (xn > 0 ? k0 + xc : 0);
   const unsigned os = xr * (unsigned)nblk + (xn > 0 ? (k0 + xc) >> 5 : 0);
+  constexpr int XL = XC >= 16 ? XC / 16 : 1, NF = YP + XL + 1;   // loads of a lane's codes, of a step
   auto fetch_piece = [&](Rows& R, const At& p, int i) {
     if (i < YP) {
       R.y[i].load_all(p.y + (long long)(i * YR) * lddy + oy);
+    } else if (i < YP + XL) {
+      if constexpr (XC >= 16) {
+        typedef unsigned u32x4_u __attribute__((ext_vector_type(4), aligned(1)));
+        const int j = 2 * (i - YP);
+        const u32x4_u c = *reinterpret_cast<const u32x4_u*>(p.c + 8 * j + oc);
+        R.x[j] = __builtin_shufflevector(c, c, 0, 1), R.x[j + 1] = __builtin_shufflevector(c, c, 2, 3);
+      } else {
+        R.x[0] = *reinterpret_cast<const u32x2_u*>(p.c + oc);
+      }
     } else {
-      R.x[i - YP] = *reinterpret_cast<const u32x2_u*>(p.c + (long long)((i - YP) * XR) * K + oc);
       // with the three bytes behind it: a byte's load would be widened, and so waited for, a step before it is used
-      R.s[i - YP] = *reinterpret_cast<const u32_u*>(p.s + (long long)((i - YP) * XR) * nblk + os);
+      R.s = *reinterpret_cast<const u32_u*>(p.s + os);
     }
   };
   auto fetch_masked = [&](Rows& R, long long m) {
@@ -184,13 +195,14 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       const long long r = m + yr + i * YR;
       R.y[i].load(dy + (r < m1 ? r : m1 - 1) * lddy + n0 + (yn > 0 ? yc : 0), r < m1 ? yn : 0);
     }
+    const long long r = m + xr;
+    const bool ok = r < m1 && xn > 0;
 #pragma unroll
-    for (int i = 0; i < XP; ++i) {
-      const long long r = m + xr + i * XR;
-      const bool ok = r < m1 && xn > 0;
-      R.x[i] = load_codes(codes + (ok ? r * K + k0 + xc : 0), ok ? xn : 0);
-      R.s[i] = ok ? scales[r * nblk + ((k0 + xc) >> 5)] : 27u;
+    for (int j = 0; j < XP; ++j) {
+      const int n = ok ? xn - 8 * j : 0;
+      R.x[j] = load_codes(codes + (n > 0 ? r * K + k0 + xc + 8 * j : 0), n);
     }
+    R.s = ok ? scales[r * nblk + ((k0 + xc) >> 5)] : 27u;
   };
   float dsum[8];
 #pragma unroll
@@ -212,9 +224,8 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       for (int p = 0; p < P; ++p)
         *reinterpret_cast<u16x8*>(ly + (buf * P + p) * BM * TN + at<TN>(yr + i * YR, yc)) = R.y[i].plane(p);
     } else {
-      const int j = i - YP;
-      const int sb = (int)(R.s[j] & 0xffu), e = F16 ? max(sb - xtop, -60) : sb - 127;      // 60 octaves below the largest nothing is left in fp16
-      *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr + j * XR, xc)) = widen<F16>(R.x[j], pow2f(e));
+      const int j = i - YP, sb = (int)(R.s & 0xffu), e = F16 ? max(sb - xtop, -60) : sb - 127;      // 60 octaves below the largest nothing is left in fp16
+      *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr, xc + 8 * j)) = widen<F16>(R.x[j], pow2f(e));
     }
   };
 
@@ -239,10 +250,10 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       F.a[p][a] = __builtin_shufflevector(tr_read(q), tr_read(q + 4 * TN), 0, 1, 2, 3, 4, 5, 6, 7);
     }
   };
-  constexpr int G = P * AN, NR = AK + P * AN, NQ = YP + XP;      // groups of AK products a substep; fragments; pieces of a step's rows
+  constexpr int G = P * AN * AK, NR = AK + P * AN, NQ = YP + XP; // products a substep; its fragments; writes of a step's rows
   auto multiply = [&](const Frags& F, int g) {
-#pragma unroll
-    for (int b = 0; b < AK; ++b) acc[g % AN][b] = mfma<F16>(F.a[g / AN][g % AN], F.b[b], acc[g % AN][b]);
+    const int p = g / (AN * AK), a = g / AK % AN, b = g % AK;
+    acc[a][b] = mfma<F16>(F.a[p][a], F.b[b], acc[a][b]);
   };
 
   // steps that need no mask: all their rows lie in the chunk, and what a lane reads behind a row's end lies in the matrix
@@ -265,15 +276,15 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
         for (int i = 0; i < NQ; ++i) stage_piece(R[u - 3], u - 3, i);
       }
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) fetch_piece(R[u % 3], next, i);
+      for (int i = 0; i < NF; ++i) fetch_piece(R[u % 3], next, i);
       advance();
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NR; ++i) read_piece(F[0], 0, 0, i);
     // step t with t % 3 == J: buffer J is multiplied, J + 1 is ready, J + 2 is written from the registers of the same number, which then take
-    // a step from memory.  The products go in groups with a share of the other work before each, in that order: left to itself the
-    // compiler puts all products of a substep behind all of its loads, and the matrix cores wait.
+    // a step from memory.  Each product is followed by a share of the other work, in that order: a wavefront issues in order, so work
+    // beside a product runs while the matrix core does, and work between groups of products (where the compiler puts it by itself) does not.
     auto step = [&](long long t, auto jc, auto fc) {
       constexpr int J = decltype(jc)::value, J1 = (J + 1) % 3, J2 = (J + 2) % 3, F0 = decltype(fc)::value;
       sum_rows(R[J2], t + 2 < nf);
@@ -284,13 +295,14 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
         for (int g = 0; g < G; ++g) {
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < NR; ++i)                           // the last group reads nothing: what it would read is needed at once
-            if (i * (G - 1) / NR == g) read_piece(nxt, st < NS - 1 ? J : J1, st < NS - 1 ? st + 1 : 0, i);
+          for (int i = 0; i < NR; ++i)                           // none beside the last quarter: what they bring is needed at once
+            if (i * (G - G / 4) / NR == g) read_piece(nxt, st < NS - 1 ? J : J1, st < NS - 1 ? st + 1 : 0, i);
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) {
+          for (int i = 0; i < NQ; ++i)
             if (st == 0 && i * G / NQ == g) stage_piece(R[J2], J2, i);
-            if (st == NS - 1 && (NS > 1 ? i * G / NQ : G - 1) == g) fetch_piece(R[J2], next, i);
-          }
+#pragma unroll
+          for (int i = 0; i < NF; ++i)
+            if (st == NS - 1 && (NS > 1 ? i * G / NF : G - 1) == g) fetch_piece(R[J2], next, i);
           multiply(cur, g);
         }
       }

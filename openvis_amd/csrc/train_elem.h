@@ -8,6 +8,7 @@
 // block.  The scale is the smallest power of two in [2^-100, 2^120] under which the block's largest finite magnitude is at most 448, so no
 // value saturates and every value above 2^-6 of its scale is off by at most 2^-4 of itself.  The limits keep scale, value and their product
 // inside f32's normal range.  e4m3 has no infinity: infinities and NaN become the NaN code and do not take part in the block's maximum.
+// (Values from 2^128 (1 - 2^-5) on round to a code that stands for 2^128, an infinity in f32.)
 #pragma once
 #include "common.h"
 

@@ -11,7 +11,7 @@
 //   dY fp16: fp16 products; X is scaled per 32 columns by the largest scale of the workgroup's rows so that its largest code comes to at most
 //   57344: exact for scales down to 2^-22 of the largest, below that off by at most 2^-30 of the 32 columns' largest value.
 // All products are exact in f32; sums are f32.  Rows are split over workgroups (S parts) where there are too few tiles to fill the card; the
-// parts are added in a fixed order by a second kernel.
+// parts are added in a fixed order by a second kernel.  36928 x 1024 x 4096 fp16: 281 us, 1.10 PFLOP/s (2000 x 1000 x 1000: 27 us).
 #include "train_elem.h"
 #include <type_traits>
 
@@ -112,7 +112,8 @@ __device__ __forceinline__ u16x8 widen(u32x2_u c, float f) {
 template <typename T, int TN, int TK, int WN, int WK, int BM>
 __global__ void __launch_bounds__(64 * WN * WK)
 wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                   float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k, int turns) {
+                   float* __restrict__ out, float* __restrict__ dbp, long long M, int N, int K, long long chunk, int tiles_n, int tiles_k, int turns,
+                   const uint8_t* __restrict__ tops, int tshift) {
   constexpr bool F16 = sizeof(T) == 2 && !__is_same(T, __bf16);
   constexpr int P = sizeof(T) == 4 ? 3 : 1, NT = 64 * WN * WK, RN = TN / WN, RK = TK / WK, AN = RN / 32, AK = RK / 32, NS = BM / 16;
   constexpr int YR = NT / (TN / 8), YP = BM / YR;                // dY: rows a pass, passes of eight columns a lane
@@ -132,18 +133,19 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   if constexpr (F16) {                                           // the largest scale of each 32 columns over the workgroup's rows
     if (tid < TK / 32) top[tid] = 27;                           // the smallest scale that the 8-bit form has
     __syncthreads();
-    // a lane reads a row's TK / 32 bytes at once (those behind the row's end belong to the next row, and to columns that are not used); the
-    // last rows, where that would leave the array, byte by byte
+    // from the scales themselves, or from the largest of 32 rows each (tops, tshift 5).  A lane reads a row's TK / 32 bytes at once (those behind
+    // the row's end belong to the next row, and to columns that are not used); the last rows, where that would leave the array, byte by byte
     typedef unsigned short pairs __attribute__((ext_vector_type(2)));
     constexpr int NB = TK / 32, NW = NB > 4 ? NB / 4 : 1;
     const int b0 = k0 >> 5;
-    const long long whole = M - 8 < m1 ? M - 8 : m1;
+    const long long up = (1ll << tshift) - 1, r0 = m0 >> tshift, r1 = (m1 + up) >> tshift, all = (M + up) >> tshift;
+    const long long whole = all - 8 < r1 ? all - 8 : r1;
     pairs hi[NW][2];
 #pragma unroll
     for (int w = 0; w < NW; ++w) hi[w][0] = hi[w][1] = (pairs)0;
 #pragma unroll 8
-    for (long long m = m0 + tid; m < whole; m += NT) {
-      const uint8_t* p = scales + m * nblk + b0;
+    for (long long m = r0 + tid; m < whole; m += NT) {
+      const uint8_t* p = tops + m * nblk + b0;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const unsigned v = NB >= 4 ? *reinterpret_cast<const u32_u*>(p + 4 * w) : *reinterpret_cast<const u16_u*>(p);
@@ -154,8 +156,8 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       int t = hi[i / 4][i & 1][(i >> 1) & 1];
-      const long long m = (whole > m0 ? whole : m0) + tid;
-      if (m < m1 && b0 + i < nblk) t = max(t, (int)scales[m * nblk + b0 + i]);
+      const long long m = (whole > r0 ? whole : r0) + tid;
+      if (m < r1 && b0 + i < nblk) t = max(t, (int)tops[m * nblk + b0 + i]);
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) t = max(t, __shfl_xor(t, o, 64));
       if (lane == 0) atomicMax(&top[i], t);                      // a maximum: the order does not matter
@@ -385,6 +387,25 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   }
 }
 
+// the largest scale of 32 rows each: tops [ceil(M / 32)][nblk].  A workgroup of the main kernel reads 8 bytes of every row's scales, a cache line
+// each: 25 us of 9232 rows.  Here the lines are read whole, once.
+__global__ void __launch_bounds__(256)
+scale_tops_kernel(const uint8_t* __restrict__ scales, uint8_t* __restrict__ tops, long long M, int nblk, long long n) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long g = i / nblk, m = g * 32;
+  const uint8_t* p = scales + m * nblk + (i - g * nblk);
+  const int rows = M - m < 32 ? (int)(M - m) : 32;
+  int t = 0;
+  if (rows == 32) {
+#pragma unroll
+    for (int r = 0; r < 32; ++r) t = max(t, (int)p[(long long)r * nblk]);
+  } else {
+    for (int r = 0; r < rows; ++r) t = max(t, (int)p[(long long)r * nblk]);
+  }
+  tops[i] = (uint8_t)t;
+}
+
 // dw = gamma sum over the parts + beta db
 __global__ void __launch_bounds__(256)
 wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict__ db, const float* __restrict__ gamma, const float* __restrict__ beta,
@@ -455,12 +476,22 @@ inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
   return best;
 }
 
+// the scales' tops by a launch of their own: where a workgroup's share is 2048 rows or more (below, its own scan is shorter than the launch)
+inline bool own_tops(const WgradShape& w, int dtype) { return dtype == OVIS_F16 && w.chunk >= 2048; }
+// the workspace: parts of dw and db, the join's sum, tops (4-byte words each)
+struct WgradSpace { long long parts, lines, sum, tops; };
+inline WgradSpace wgrad_space(const WgradShape& w, long long M, int N, int K, int dtype) {
+  const long long NK = (long long)N * K;
+  return {w.S * NK, (long long)w.S * w.turns * N, NK < 65536 ? NK : 0, own_tops(w, dtype) ? (M + 31) / 32 * ((K + 31) / 32) / 4 + 1 : 0};
+}
+
 }  // namespace
 
 extern "C" long long ovis_linear_wgrad_ckpt8_workspace_bytes(long long M, int N, int K, int dtype) {
   if (M <= 0 || N <= 0 || K <= 0 || !ovis::dtype_ok(dtype)) return 0;
   const WgradShape w = wgrad_shape(M, N, K, dtype);
-  return ((long long)w.S * N * K + (long long)w.S * w.turns * N + ((long long)N * K < 65536 ? (long long)N * K : 0)) * 4;
+  const WgradSpace p = wgrad_space(w, M, N, K, dtype);
+  return (p.parts + p.lines + p.sum + p.tops) * 4;
 }
 
 extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, const float* gamma,
@@ -476,7 +507,18 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
   const bool join = w.S > 1 || gamma;
   float* part = join ? workspace : dw;
   const int lines = w.S * w.turns;
-  float* dbp = lines > 1 ? workspace + (long long)w.S * N * K : db;
+  const WgradSpace sp = wgrad_space(w, M, N, K, dtype);
+  float* dbp = lines > 1 ? workspace + sp.parts : db;
+  const uint8_t* tops = scales;
+  int tshift = 0;
+  if (own_tops(w, dtype)) {
+    uint8_t* t = (uint8_t*)(workspace + sp.parts + sp.lines + sp.sum);
+    const long long n = (M + 31) / 32 * ((K + 31) / 32);
+    hipLaunchKernelGGL(scale_tops_kernel, dim3(ovis::cdiv(n, 256)), dim3(256), 0, (hipStream_t)stream, scales, t, M, (K + 31) / 32, n);
+    const int rc = ovis::check_launch("linear_wgrad_ckpt8");
+    if (rc != OVIS_OK) return rc;
+    tops = t, tshift = 5;
+  }
 #define WG_GO(T, TN, TK, WN, WK, BM)                                                                                                        \
   {                                                                                                                                         \
     const int lds = 3 * BM * (TN * (sizeof(T) == 4 ? 3 : 1) + TK) * 2;                                                                      \
@@ -486,7 +528,7 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
       if (e != hipSuccess) return ovis::fail(OVIS_ELAUNCH, "linear_wgrad_ckpt8: %s", hipGetErrorString(e));                                 \
     }                                                                                                                                       \
     hipLaunchKernelGGL((wgrad_ckpt8_kernel<T, TN, TK, WN, WK, BM>), dim3((unsigned)blocks), dim3(64 * WN * WK), lds, (hipStream_t)stream,   \
-                       (const T*)dy, lddy, codes, scales, part, dbp, M, N, K, w.chunk, w.tiles_n, w.tiles_k, w.turns);                      \
+                       (const T*)dy, lddy, codes, scales, part, dbp, M, N, K, w.chunk, w.tiles_n, w.tiles_k, w.turns, tops, tshift);        \
   }
   if (dtype == OVIS_F32) {
     if (w.tile == 128) WG_GO(float, 128, 128, 2, 2, 16)
@@ -507,7 +549,7 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
   const long long NK = (long long)N * K;
   int S = w.S;
   if (S > 8 && NK < 65536) {                                     // few columns, many parts: 64 lanes a column (9000 x 64 x 64 in 141 parts: 57 us by one)
-    float* to = gamma ? workspace + (long long)w.S * NK + (long long)lines * N : dw;
+    float* to = gamma ? workspace + sp.parts + sp.lines : dw;
     rc = ovis::column_sum_finish(part, S, (int)NK, to, (int)NK, to, (hipStream_t)stream);
     if (rc != OVIS_OK || !gamma) return rc;
     part = to;

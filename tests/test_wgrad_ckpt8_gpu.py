@@ -18,7 +18,7 @@ def _value8(ck):
 
 
 SHAPES = [(1, 1, 1), (1, 3, 5), (7, 8, 32), (63, 64, 64), (64, 65, 33), (65, 33, 65), (100, 256, 2048), (197, 129, 257), (300, 100, 1000), (1000, 64, 48),
-          (4097, 72, 200), (5000, 384, 96), (20000, 8, 16), (2500, 768, 768), (9000, 1030, 520), (33000, 256, 512)]
+          (4097, 72, 200), (5000, 384, 96), (20000, 8, 16), (2500, 768, 768), (9000, 1030, 520), (33000, 256, 512), (9000, 2048, 2100), (70001, 1000, 1000)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)

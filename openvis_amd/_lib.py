@@ -100,29 +100,6 @@ def call(name, *args):
         _throttle()
 
 
-_ENTRIES = {}
-_CTYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
-
-
-def entry(name, signature, returns="i"):
-    """The ovis_* function `name` with declared argument types (p pointer, i int, l long long, f float), made once: it takes plain ints (None = a
-    null pointer), which costs a small call a few microseconds less than converting argument by argument."""
-    fn = _ENTRIES.get(name)
-    if fn is None:
-        proto = ctypes.CFUNCTYPE(_CTYPES[returns], *[_CTYPES[c] for c in signature])      # a prototype of its own: call() leaves types open
-        fn = _ENTRIES[name] = proto((name, lib()))
-    return fn
-
-
-def run(name, signature, *args):
-    """entry(name, signature)(*args); raise OvisError on a non-zero code."""
-    rc = entry(name, signature)(*args)
-    if rc != 0:
-        raise OvisError(f"{name} failed (code {rc}): {lib().ovis_last_error().decode()}")
-    if LAUNCH_WINDOW > 0:
-        _throttle()
-
-
 _raw_stream = None
 
 
@@ -140,9 +117,3 @@ def stream_ptr():
             _raw_stream = lambda: torch.cuda.current_stream().cuda_stream
     return ctypes.c_void_p(_raw_stream())
 
-
-def raw_stream():
-    """stream_ptr() as an int, for entry()"""
-    if _raw_stream is None:
-        stream_ptr()
-    return _raw_stream()

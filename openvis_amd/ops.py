@@ -17,12 +17,12 @@ _EXT = None
 
 
 def _mi():
-    """torch.ops.ovis_mi: the dispatcher ops of the hot stages (csrc/torch_ext/hot_ops.cpp + msda_module.cpp, registered when the
+    """torch.ops.ovis_mi: the dispatcher ops of the hot stages (csrc/torch_ext/{hot_ops,train_ops,msda_module}.cpp, registered when the
     compiled extension `MultiScaleDeformableAttention` is imported).  A missing build fails loudly, with the build hint."""
     global _EXT
     if _EXT is None:
         from .modeling.pixel_decoder.ops.functions import ms_deform_attn_func      # imports the extension (or raises the hint)
-        if not hasattr(torch.ops.ovis_mi, "gemm_nt_f16"):
+        if not (hasattr(torch.ops.ovis_mi, "gemm_nt_f16") and hasattr(torch.ops.ovis_mi, "layernorm_forward")):
             raise _lib.OvisError("the compiled extension lacks the ovis_mi hot ops: rebuild it (python -c 'import __graft_entry__ as g; g.build()')")
         _EXT = torch.ops.ovis_mi
     return _EXT
@@ -1039,14 +1039,11 @@ def gemm_nt_planes(a3, w3, bias=None, residual=None, act=ACT_NONE, out_planes=Fa
     return out
 
 
-# ---- training-side operators (csrc/layernorm_train.hip, relpos.hip, act_ckpt8.hip, wgrad_ckpt8.hip; include/openvis_hip.h) --------------
+# ---- training-side operators (csrc/layernorm_train.hip, relpos.hip, act_ckpt8.hip, wgrad_ckpt8.hip; csrc/torch_ext/train_ops.cpp) ---------
 # Forward passes that keep what the backward pass needs, and the backward passes, as plain functions: they take and return tensors and
 # build no autograd graph.  f32 / fp16 / bf16 tensors, f32 arithmetic, sums in a fixed order (the same bits at every call).  Rows may be
-# strided (a slice of wider rows); the elements of a row are contiguous.  Workspaces come from torch's allocator at every call, so calls on
-# several streams, or in several captured graphs, share nothing.
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-
-
+# strided (a slice of wider rows); the elements of a row are contiguous.  Tensors lie on one device, whose current stream the kernels are queued
+# on.  Workspaces come from torch's allocator at every call, so calls on several streams, or in several captured graphs, share nothing.
 class Ckpt8(typing.NamedTuple):
     """A matrix [rows, C] in 8 bits: codes float8_e4m3fn [rows, C] and one power-of-two scale per 32 columns, float8_e8m0fnu
     [rows, ceil(C / 32)].  It stands for codes * scales."""
@@ -1061,212 +1058,75 @@ class LayerNormForward(typing.NamedTuple):
     xhat8: typing.Optional[Ckpt8]
 
 
-def _train_check(name, *tensors):
-    """every tensor on the current HIP device: kernels are queued on that device's current stream"""
-    cur = None
-    for t in tensors:
-        if t is not None:
-            d = t.get_device()
-            if cur is None:
-                cur = torch.cuda.current_device() if d >= 0 else -1
-            if d < 0 or d != cur:
-                raise _lib.OvisError(f"{name}: tensors must be on the current HIP device (got {t.device}; no CPU fallback)")
-
-
-def _train_dtype(name, what, t):
-    d = _DTYPES.get(t if isinstance(t, torch.dtype) else t.dtype)
-    if d is None:
-        raise _lib.OvisError(f"{name}: {what} must be float32, float16 or bfloat16")
-    return d
-
-
-def _train_rows(name, what, t, C):
-    """(rows, row stride in elements) of t [..., C]"""
-    if t.dim() < 1 or t.shape[-1] != C or C < 1:
-        raise _lib.OvisError(f"{name}: {what} must be [..., {C}], got {tuple(t.shape)}")
-    if t.is_contiguous():
-        return t.numel() // C, C
+def _train(op, *args):
+    """a dispatcher op of csrc/torch_ext/train_ops.cpp; what it refuses is an OvisError (running out of memory stays torch's own error)"""
     try:
-        v = t.view(-1, C)
-    except RuntimeError:
-        v = None
-    if v is None or (C > 1 and v.stride(1) != 1) or (v.shape[0] > 1 and v.stride(0) < C):
-        raise _lib.OvisError(f"{name}: {what} needs contiguous elements in rows that are one stride apart (got strides {tuple(t.stride())})")
-    return v.shape[0], (v.stride(0) if v.shape[0] > 1 else C)
-
-
-def _train_vec(name, what, t, C):
-    if t.dtype != torch.float32 or t.numel() != C or not t.is_contiguous():
-        raise _lib.OvisError(f"{name}: {what} must be a contiguous float32 vector of {C}")
-
-
-def _train_ckpt(name, ck):
-    codes, scales = ck
-    if (codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float8_e8m0fnu or codes.dim() != 2 or not codes.is_contiguous()
-            or not scales.is_contiguous() or codes.shape[1] < 1 or tuple(scales.shape) != (codes.shape[0], (codes.shape[1] + 31) // 32)):
-        raise _lib.OvisError(f"{name}: a Ckpt8 holds contiguous float8_e4m3fn codes [rows, C] and float8_e8m0fnu scales [rows, ceil(C / 32)]")
-    return codes.shape
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _like(t, dtype):
-    """an uninitialised contiguous tensor of t's shape (the first form costs half a microsecond less)"""
-    return torch.empty_like(t) if t.dtype == dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
-
-
-def _workspace(name, signature, device, *args):
-    """f32 workspace of the size that the library asks for"""
-    return torch.empty((_lib.entry(name, signature, "l")(*args) // 4,), dtype=torch.float32, device=device)
-
-
-def _new_ckpt(rows, C, device):
-    return Ckpt8(torch.empty((rows, C), dtype=torch.float8_e4m3fn, device=device),
-                 torch.empty((rows, (C + 31) // 32), dtype=torch.float8_e8m0fnu, device=device))
+        return getattr(_mi(), op)(*args)
+    except RuntimeError as e:
+        if type(e) is not RuntimeError:
+            raise
+        raise _lib.OvisError(str(e).partition("\nException raised from")[0]) from None
 
 
 def layernorm_forward(x, gamma, beta, residual=None, eps=1e-5, out_dtype=None, checkpoint=False):
     """layernorm() for training: x [..., C] (+ residual of the same shape and type) -> LayerNormForward(y, sum, stats, xhat8).
     y has out_dtype (x's type, or any of the three where x is f32); checkpoint=True also keeps the normalised rows in 8 bits, from which
     layernorm_backward and linear_wgrad_ckpt8 work without x.  C <= 8192.  The reference trains nn.LayerNorm, msdeformattn.py:139-146."""
-    name = "layernorm_forward"
-    C = x.shape[-1] if x.dim() else 0
-    _train_check(name, x, gamma, beta, residual)
-    xd = _train_dtype(name, "x", x)
-    yd = xd if out_dtype is None else _train_dtype(name, "out_dtype", out_dtype)
-    rows, ldx = _train_rows(name, "x", x, C)
-    ldr = 0
-    if residual is not None:
-        if residual.dtype != x.dtype or residual.shape != x.shape:
-            raise _lib.OvisError(f"{name}: residual must have x's shape and type")
-        ldr = _train_rows(name, "residual", residual, C)[1]
-    _train_vec(name, "gamma", gamma, C)
-    _train_vec(name, "beta", beta, C)
-    y = _like(x, x.dtype if out_dtype is None else out_dtype)
-    total = _like(x, x.dtype) if residual is not None else x
-    stats = gamma.new_empty((rows, 2))
-    ck = _new_ckpt(rows, C, x.device) if checkpoint else None
-    if rows:
-        _lib.run("ovis_layernorm_train_forward", "plplppppppplifiip", x.data_ptr(), ldx, _ptr(residual), ldr, gamma.data_ptr(), beta.data_ptr(),
-                 total.data_ptr() if residual is not None else None, y.data_ptr(), stats.data_ptr(), ck.codes.data_ptr() if ck else None,
-                 ck.scales.data_ptr() if ck else None, rows, C, float(eps), xd, yd, _lib.raw_stream())
-    return LayerNormForward(y, total, stats, ck)
+    y, total, stats, codes, scales = _train("layernorm_forward", x, gamma, beta, residual, eps, out_dtype, checkpoint)
+    return LayerNormForward(y, x if residual is None else total, stats, Ckpt8(codes, scales) if checkpoint else None)
 
 
 def layernorm_backward(dy, x, stats, gamma, dsum=None, out_dtype=None):
     """Gradients of layernorm_forward: (dx, dgamma, dbeta), dgamma / dbeta in f32.  x: the rows that were normalised (`sum`), or `xhat8`; dsum: the
     gradient that reaches those rows past the norm, added to dx.  dx has out_dtype (default: x's type, or dsum's, or dy's with an 8-bit x)."""
-    name = "layernorm_backward"
-    ck = x if isinstance(x, Ckpt8) else None
-    C = dy.shape[-1] if dy.dim() else 0
-    _train_check(name, dy, stats, gamma, dsum, *(ck if ck else (x,)))
-    dyd = _train_dtype(name, "dy", dy)
-    rows, lddy = _train_rows(name, "dy", dy, C)
-    ldx = 0
-    if ck is not None:
-        if tuple(_train_ckpt(name, ck)) != (rows, C):
-            raise _lib.OvisError(f"{name}: the 8-bit rows are {tuple(ck.codes.shape)}, dy has {rows} rows of {C}")
-        xdt = out_dtype if out_dtype is not None else dsum.dtype if dsum is not None else dy.dtype
-    else:
-        xrows, ldx = _train_rows(name, "x", x, C)
-        if xrows != rows:
-            raise _lib.OvisError(f"{name}: x has {xrows} rows, dy {rows}")
-        xdt = x.dtype
-        if out_dtype is not None and out_dtype != xdt:
-            raise _lib.OvisError(f"{name}: dx has x's type")
-    xd = _train_dtype(name, "x / dx", xdt)
-    if xd != 0 and xd != dyd:
-        raise _lib.OvisError(f"{name}: dy has dx's type, or any where dx is f32")
-    lds = 0
-    if dsum is not None:
-        srows, lds = _train_rows(name, "dsum", dsum, C)
-        if dsum.dtype != xdt or srows != rows:
-            raise _lib.OvisError(f"{name}: dsum must have dx's type and rows")
-    if stats.dtype != torch.float32 or stats.numel() != 2 * rows or not stats.is_contiguous():
-        raise _lib.OvisError(f"{name}: stats must be contiguous float32 [{rows}, 2]")
-    _train_vec(name, "gamma", gamma, C)
-    dx = _like(dy, xdt)
-    if not rows:
-        return dx, torch.zeros((C,), dtype=torch.float32, device=dy.device), torch.zeros((C,), dtype=torch.float32, device=dy.device)
-    grads = gamma.new_empty((2, C))
-    ws = _workspace("ovis_layernorm_train_backward_workspace_bytes", "lii", dy.device, rows, C, xd)
-    dgamma, dbeta = grads.unbind(0)
-    _lib.run("ovis_layernorm_train_backward", "plplppppplppppliiip", dy.data_ptr(), lddy, x.data_ptr() if ck is None else None, ldx,
-             ck.codes.data_ptr() if ck else None, ck.scales.data_ptr() if ck else None, stats.data_ptr(), gamma.data_ptr(), _ptr(dsum), lds,
-             dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), rows, C, dyd, xd, _lib.raw_stream())
-    return dx, dgamma, dbeta
+    if isinstance(x, tuple):
+        return _train("layernorm_backward", dy, None, x[0], x[1], stats, gamma, dsum, out_dtype)
+    return _train("layernorm_backward", dy, x, None, None, stats, gamma, dsum, out_dtype)
 
 
 def ckpt8_encode(x):
     """x [..., C] in 8 bits, its leading dimensions as rows: Ckpt8.  Values are off by at most 2^-4 of themselves (2^-10 of the block's scale
     below 2^-6 of it); NaN and infinities become NaN."""
-    return _act_ckpt8("ckpt8_encode", x, ACT_NONE)[1]
+    return Ckpt8(*_train("act_forward_ckpt8", x, ACT_NONE)[1:])
 
 
 def ckpt8_decode(ck, dtype=torch.float32):
     """the values [rows, C] that a Ckpt8 stands for, in `dtype`"""
-    name = "ckpt8_decode"
-    _train_check(name, *ck)
-    rows, C = _train_ckpt(name, ck)
-    d = _train_dtype(name, "dtype", dtype)
-    out = torch.empty((rows, C), dtype=dtype, device=ck.codes.device)
-    if rows:
-        _lib.run("ovis_ckpt8_decode", "pppliip", ck.codes.data_ptr(), ck.scales.data_ptr(), out.data_ptr(), rows, C, d, _lib.raw_stream())
-    return out
+    return _train("ckpt8_decode", ck[0], ck[1], dtype)
 
 
 def act_forward_ckpt8(h, act):
     """The activation of an MLP (ACT_RELU, ACT_QUICKGELU or ACT_GELU), for training: h [..., C] -> (y = act(h) in h's type, h as a Ckpt8)."""
-    if act not in (ACT_RELU, ACT_QUICKGELU, ACT_GELU):
+    if act == ACT_NONE:
         raise _lib.OvisError("act_forward_ckpt8: act must be ACT_RELU, ACT_QUICKGELU or ACT_GELU")
-    return _act_ckpt8("act_forward_ckpt8", h, act)
-
-
-def _act_ckpt8(name, h, act):
-    C = h.shape[-1] if h.dim() else 0
-    _train_check(name, h)
-    d = _train_dtype(name, "input", h)
-    rows, ldh = _train_rows(name, "input", h, C)
-    y = _like(h, h.dtype) if act else None
-    ck = _new_ckpt(rows, C, h.device)
-    if rows:
-        _lib.run("ovis_act_ckpt8_forward", "plpppliiip", h.data_ptr(), ldh, _ptr(y), ck.codes.data_ptr(), ck.scales.data_ptr(), rows, C, int(act), d,
-                 _lib.raw_stream())
-    return y, ck
+    y, codes, scales = _train("act_forward_ckpt8", h, act)
+    return y, Ckpt8(codes, scales)
 
 
 def act_backward_ckpt8(dy, h8, act, recompute=False):
     """Gradient of act_forward_ckpt8: dy [..., C] and the 8-bit h -> (dh in dy's type, dbias f32 [C] = column sums of dh -- the gradient of the
     bias of the linear layer that made h --, act(h8) as a Ckpt8 if recompute, else None: the operand of the next layer's weight gradient)."""
-    name = "act_backward_ckpt8"
-    if act not in (ACT_RELU, ACT_QUICKGELU, ACT_GELU):
-        raise _lib.OvisError(f"{name}: act must be ACT_RELU, ACT_QUICKGELU or ACT_GELU")
-    _train_check(name, dy, *h8)
-    rows, C = _train_ckpt(name, h8)
-    d = _train_dtype(name, "dy", dy)
-    drows, lddy = _train_rows(name, "dy", dy, C)
-    if drows != rows:
-        raise _lib.OvisError(f"{name}: dy has {drows} rows, the 8-bit rows are {rows}")
-    dh = _like(dy, dy.dtype)
-    y8 = _new_ckpt(rows, C, dy.device) if recompute else None
-    if not rows:
-        return dh, torch.zeros((C,), dtype=torch.float32, device=dy.device), y8
-    dbias = torch.empty((C,), dtype=torch.float32, device=dy.device)
-    ws = _workspace("ovis_act_ckpt8_backward_workspace_bytes", "li", dy.device, rows, C)
-    _lib.run("ovis_act_ckpt8_backward", "plpppppppliiip", dy.data_ptr(), lddy, h8.codes.data_ptr(), h8.scales.data_ptr(), dh.data_ptr(),
-             dbias.data_ptr(), y8.codes.data_ptr() if y8 else None, y8.scales.data_ptr() if y8 else None, ws.data_ptr(), rows, C, int(act), d,
-             _lib.raw_stream())
-    return dh, dbias, y8
+    dh, dbias, codes, scales = _train("act_backward_ckpt8", dy, h8[0], h8[1], act, recompute)
+    return dh, dbias, Ckpt8(codes, scales) if recompute else None
+
+
+def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
+    """Gradients of a linear layer's weight [N, K] and bias [N] (f32): dy [..., N] and the layer's input as a Ckpt8 [rows, K] -> (dw, db).  With a
+    layer norm's gamma / beta [K], x8 is its xhat8 and the layer's input was xhat * gamma + beta."""
+    return _train("linear_wgrad_ckpt8", dy, x8[0], x8[1], gamma, beta)
 
 
 @functools.lru_cache(maxsize=64)
 def _relpos_borders(num_buckets, max_distance, bidirectional):
-    """distances at which the buckets of a direction begin (bucket 0 is distance 0), counted in whole numbers: with n = the direction's
-    buckets and e = n // 2, bucket k < e is distance k; bucket e + k begins at the first d with (d / e)^(n - e) >= (max_distance / e)^k."""
+    """int32 tensor on the host: the distances at which the buckets of a direction begin (bucket 0 is distance 0), counted in whole numbers: with
+    n = the direction's buckets and e = n // 2, bucket k < e is distance k; bucket e + k begins at the first d with
+    (d / e)^(n - e) >= (max_distance / e)^k."""
     n = num_buckets // 2 if bidirectional else num_buckets
     e = n // 2
+    if n < 2 or n > 257 or (bidirectional and num_buckets % 2):
+        raise _lib.OvisError(f"relpos_bias_1d: 2 to 257 buckets a direction, an even number in all with two directions (got {num_buckets})")
+    if not e < max_distance < 2 ** 30:
+        raise _lib.OvisError(f"relpos_bias_1d: max_distance must be more than the {e} distances with a bucket of their own, and less than 2^30")
     at = list(range(1, e + 1))
     for k in range(1, n - e):
         lo, hi = at[-1], max_distance                 # the border is at most max_distance: (max_distance / e)^(n - e - k) >= 1
@@ -1277,114 +1137,29 @@ def _relpos_borders(num_buckets, max_distance, bidirectional):
             else:
                 lo = m + 1
         at.append(lo)
-    return (ctypes.c_int * len(at))(*at), len(at)
-
-
-def _relpos_args(name, num_buckets, max_distance, bidirectional, q_offset):
-    num_buckets, max_distance, q_offset = int(num_buckets), int(max_distance), int(q_offset)
-    n = num_buckets // 2 if bidirectional else num_buckets
-    if n < 2 or n > 257 or (bidirectional and num_buckets % 2):
-        raise _lib.OvisError(f"{name}: 2 to 257 buckets a direction, an even number in all with two directions (got {num_buckets})")
-    if not n // 2 < max_distance < 2 ** 30:
-        raise _lib.OvisError(f"{name}: max_distance must be more than the {n // 2} distances with a bucket of their own, and less than 2^30")
-    if abs(q_offset) >= 2 ** 60:
-        raise _lib.OvisError(f"{name}: q_offset {q_offset}")
-    return (*_relpos_borders(num_buckets, max_distance, bool(bidirectional)), q_offset)
+    return torch.tensor(at, dtype=torch.int32)
 
 
 def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset=0, out_dtype=torch.float32, ld=None):
     """Relative position bias of a sequence by buckets: table f32 [buckets, H] -> [H, Nq, Nk] with bias[h,i,j] = table[bucket(j - i - q_offset), h]
     (a view of rows padded with zeros to 16 bytes), or with ld the padded rows themselves, [H, Nq, ld], as attention(bias=...,
-    bias_strides=(0, Nq * ld)) takes them.  A distance below half of a direction's buckets has a bucket of its own; the others grow logarithmically up to max_distance, the last bucket
-    holds all that is farther.  bidirectional: the second half of the buckets is for keys behind the query (j > i + q_offset); otherwise
-    those have distance 0.  q_offset: position of the first query among the keys (one new token of a cache: Nq = 1, q_offset = Nk - 1)."""
-    name = "relpos_bias_1d"
-    _train_check(name, table)
-    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous() or table.shape[1] < 1:
-        raise _lib.OvisError(f"{name}: table must be contiguous float32 [buckets, heads]")
-    borders, nb, off = _relpos_args(name, table.shape[0], max_distance, bidirectional, q_offset)
-    d = _train_dtype(name, "out_dtype", out_dtype)
-    Nq, Nk, H = int(Nq), int(Nk), table.shape[1]
-    if Nq < 0 or Nk < 0:
-        raise _lib.OvisError(f"{name}: Nq {Nq}, Nk {Nk}")
-    v = 4 if d == 0 else 8
-    row = (Nk + v - 1) // v * v if ld is None else int(ld)
-    if row < Nk or row % v:
-        raise _lib.OvisError(f"{name}: ld must be at least {Nk} and a multiple of {v}")
-    out = table.new_empty((H, Nq, row), dtype=out_dtype)
-    if Nq and Nk:
-        _lib.run("ovis_relpos_bias_1d", "pppiiiiiilip", table.data_ptr(), out.data_ptr(), borders, nb, int(bool(bidirectional)), H, Nq, Nk, row, off, d,
-                 _lib.raw_stream())
-    elif row:
-        out.zero_()
-    return out if ld is not None or row == Nk else out[..., :Nk]
-
-
-def _relpos_grad(name, dbias):
-    """dbias [H, Nq, Nk] or [B, H, Nq, Nk] with contiguous elements -> (B, H, Nq, Nk, strides, type)"""
-    _train_check(name, dbias)
-    d = _train_dtype(name, "dbias", dbias)
-    g = dbias[None] if dbias.dim() == 3 else dbias
-    if g.dim() != 4 or g.shape[1] < 1 or (g.shape[3] > 1 and g.stride(3) != 1):
-        raise _lib.OvisError(f"{name}: dbias must be [H, Nq, Nk] or [B, H, Nq, Nk] with contiguous rows (got {tuple(dbias.shape)}, strides {tuple(dbias.stride())})")
-    return (*g.shape, *g.stride()[:3], d)
+    bias_strides=(0, Nq * ld)) takes them.  A distance below half of a direction's buckets has a bucket of its own; the others grow
+    logarithmically up to max_distance, the last bucket holds all that is farther.  bidirectional: the second half of the buckets is for keys
+    behind the query (j > i + q_offset); otherwise those have distance 0.  q_offset: position of the first query among the keys (one new token of
+    a cache: Nq = 1, q_offset = Nk - 1)."""
+    borders = _relpos_borders(table.shape[0] if table.dim() else 0, int(max_distance), bool(bidirectional))
+    if ld is not None and ld < max(Nk, 1):
+        raise _lib.OvisError(f"relpos_bias_1d: ld must be at least {max(Nk, 1)}")
+    return _train("relpos_bias_1d", table, borders, bool(bidirectional), Nq, Nk, q_offset, out_dtype, ld or 0)
 
 
 def relpos_bias_1d_backward(dbias, num_buckets, max_distance=128, bidirectional=True, q_offset=0):
     """Gradient of relpos_bias_1d's table, f32 [num_buckets, H]: dbias [H, Nq, Nk] or [B, H, Nq, Nk] (the bias is shared by the batch; f32, fp16
     or bf16, any strides but the last) summed over the batch and over the pairs of each bucket."""
-    name = "relpos_bias_1d_backward"
-    B, H, Nq, Nk, bs, hs, ld, d = _relpos_grad(name, dbias)
-    borders, nb, off = _relpos_args(name, num_buckets, max_distance, bidirectional, q_offset)
-    if not (B and Nq and Nk):
-        return torch.zeros((num_buckets, H), dtype=torch.float32, device=dbias.device)
-    out = torch.empty((num_buckets, H), dtype=torch.float32, device=dbias.device)
-    ws = _workspace("ovis_relpos_bias_1d_backward_workspace_bytes", "liii", dbias.device, B, H, Nq, Nk)
-    _lib.run("ovis_relpos_bias_1d_backward", "plllpppiiliiilip", dbias.data_ptr(), bs, hs, ld, out.data_ptr(), ws.data_ptr(), borders, nb,
-             int(bool(bidirectional)), B, H, Nq, Nk, off, d, _lib.raw_stream())
-    return out
+    return _train("relpos_bias_1d_backward", dbias, _relpos_borders(int(num_buckets), int(max_distance), bool(bidirectional)), bool(bidirectional), q_offset)
 
 
 def swin_relpos_bias_backward(dbias, ws):
     """Gradient of swin_relpos_bias's table, f32 [(2 ws - 1)^2, heads]: dbias [heads, N, >= N] or [B, heads, N, >= N] (N = ws * ws; columns from N
     on are padding and not read), summed over the B windows and over the token pairs of each offset (swin.py:147-155)."""
-    name = "swin_relpos_bias_backward"
-    ws = int(ws)
-    if not 1 <= ws <= 64:
-        raise _lib.OvisError(f"{name}: window size {ws} (1 to 64)")
-    B, H, N, ld_cols, bs, hs, ld, d = _relpos_grad(name, dbias)
-    if N != ws * ws or ld_cols < N:
-        raise _lib.OvisError(f"{name}: dbias must be [..., {ws * ws}, at least {ws * ws}], got {tuple(dbias.shape)}")
-    if not B:
-        return torch.zeros(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
-    out = torch.empty(((2 * ws - 1) ** 2, H), dtype=torch.float32, device=dbias.device)
-    work = _workspace("ovis_swin_relpos_bias_backward_workspace_bytes", "lii", dbias.device, B, H, ws)
-    _lib.run("ovis_swin_relpos_bias_backward", "plllppliiip", dbias.data_ptr(), bs, hs, ld, out.data_ptr(), work.data_ptr(), B, H, ws, d,
-             _lib.raw_stream())
-    return out
-
-
-def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
-    """Gradients of a linear layer's weight [N, K] and bias [N] (f32): dy [..., N] and the layer's input as a Ckpt8 [rows, K] -> (dw, db).  With a
-    layer norm's gamma / beta [K], x8 is its xhat8 and the layer's input was xhat * gamma + beta."""
-    name = "linear_wgrad_ckpt8"
-    N = dy.shape[-1] if dy.dim() else 0
-    _train_check(name, dy, *x8, gamma, beta)
-    rows, K = _train_ckpt(name, x8)
-    d = _train_dtype(name, "dy", dy)
-    drows, lddy = _train_rows(name, "dy", dy, N)
-    if drows != rows:
-        raise _lib.OvisError(f"{name}: dy has {drows} rows, the 8-bit rows are {rows}")
-    if (gamma is None) != (beta is None):
-        raise _lib.OvisError(f"{name}: gamma and beta go together")
-    if gamma is not None:
-        _train_vec(name, "gamma", gamma, K)
-        _train_vec(name, "beta", beta, K)
-    if not rows:
-        return torch.zeros((N, K), dtype=torch.float32, device=dy.device), torch.zeros((N,), dtype=torch.float32, device=dy.device)
-    dw = torch.empty((N, K), dtype=torch.float32, device=dy.device)
-    db = torch.empty((N,), dtype=torch.float32, device=dy.device)
-    ws = _workspace("ovis_linear_wgrad_ckpt8_workspace_bytes", "liii", dy.device, rows, N, K, d)
-    _lib.run("ovis_linear_wgrad_ckpt8", "plpppppppliiip", dy.data_ptr(), lddy, x8.codes.data_ptr(), x8.scales.data_ptr(), _ptr(gamma), _ptr(beta),
-             dw.data_ptr(), db.data_ptr(), ws.data_ptr(), rows, N, K, d, _lib.raw_stream())
-    return dw, db
+    return _train("swin_relpos_bias_backward", dbias, ws)

@@ -1,6 +1,5 @@
-"""CPU: what the training-side operators check before any device work, their declared signatures, and the bucket borders."""
+"""CPU: what the training-side operators check before any device work, the shapes they give, and the bucket borders."""
 import ctypes
-import inspect
 import math
 import re
 
@@ -22,19 +21,15 @@ def _prototypes():
     return out
 
 
-def test_declared_signatures_are_those_of_the_header():
-    src, protos = inspect.getsource(ops), _prototypes()
-    runs = re.findall(r'_lib\.run\("(ovis_[a-z0-9_]+)", "([pilf]+)"', src)
-    sizes = re.findall(r'_workspace\("(ovis_[a-z0-9_]+)", "([pilf]+)"', src)
-    assert len(runs) >= 8 and len(sizes) >= 5
-    for name, sig in runs:
-        assert protos[name] == ("i", sig), name
-    for name, sig in sizes:
-        assert protos[name] == ("l", sig), name
+def _entry(name, signature, returns="i"):
+    """the C function with the argument types of its prototype in the header"""
+    assert _prototypes()[name] == (returns, signature), name
+    t = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+    return ctypes.CFUNCTYPE(t[returns], *[t[c] for c in signature])((name, _lib.lib()))
 
 
 def _refused(name, sig, *args):
-    rc = _lib.entry(name, sig)(*args)
+    rc = _entry(name, sig)(*args)
     assert rc == 1, (name, rc)
     return _lib.lib().ovis_last_error().decode()
 
@@ -55,7 +50,7 @@ def test_layernorm_entry_points_refuse():
                                ("dy", "ldd", "x", "ldx", "co", "sc", "st", "g", "ds", "lds", "dx", "dg", "db", "ws", "rows", "C", "yt", "xt", "s")])
     assert "exactly one" in bwd(x=None) and "exactly one" in bwd(co=P, sc=P) and "null" in bwd(ws=None) and "null" in bwd(sc=P)
     assert "stride" in bwd(ldd=3) and "stride" in bwd(ds=P, lds=1) and "type" in bwd(xt=1, yt=2) and "columns" in bwd(rows=-1)
-    assert _lib.entry("ovis_layernorm_train_backward_workspace_bytes", "lii", "l")(0, 64, 0) == 0
+    assert _entry("ovis_layernorm_train_backward_workspace_bytes", "lii", "l")(0, 64, 0) == 0
 
 
 def test_activation_and_8_bit_entry_points_refuse():
@@ -110,7 +105,8 @@ def test_tensors_on_the_host_are_refused():
 @pytest.mark.parametrize("num,dist,both", [(32, 128, True), (32, 128, False), (8, 64, True), (64, 1000, True), (2, 2, False), (4, 2, True), (257, 100000, False)])
 def test_bucket_borders(num, dist, both):
     """against the logarithm, away from where rounding could decide: bucket = e + floor(log(d / e) / log(dist / e) * (n - e))"""
-    at, cnt = ops._relpos_borders(num, dist, both)
+    at = ops._relpos_borders(num, dist, both).tolist()
+    cnt = len(at)
     n = num // 2 if both else num
     e = n // 2
     assert cnt == n - 1 and list(at) == sorted(at) and at[0] >= 1 and at[cnt - 1] <= dist
@@ -124,3 +120,49 @@ def test_bucket_borders(num, dist, both):
                 assert mine == min(n - 1, int(v)), d
             else:                                    # a whole number by rights
                 assert mine == min(n - 1, round(v)), d
+
+
+def test_meta_tensors_give_shapes_and_types():
+    m = lambda *s, t=torch.float16: torch.empty(*s, dtype=t, device="meta")
+    g = m(96, t=torch.float32)
+    o = ops.layernorm_forward(m(3, 5, 96), g, g, residual=m(3, 5, 96), checkpoint=True)
+    assert o.y.shape == o.sum.shape == (3, 5, 96) and o.stats.shape == (15, 2) and o.xhat8.codes.shape == (15, 96) and o.xhat8.scales.shape == (15, 3)
+    dx, dg, db = ops.layernorm_backward(m(3, 5, 96), o.xhat8, o.stats, g, out_dtype=torch.float32)
+    assert dx.shape == (3, 5, 96) and dx.dtype == torch.float32 and dg.shape == db.shape == (96,)
+    y, h8 = ops.act_forward_ckpt8(m(15, 40), ops.ACT_GELU)
+    dh, dbias, y8 = ops.act_backward_ckpt8(m(15, 40), h8, ops.ACT_GELU, recompute=True)
+    assert y.shape == dh.shape == (15, 40) and dbias.shape == (40,) and y8.scales.shape == (15, 2)
+    dw, db = ops.linear_wgrad_ckpt8(m(15, 7), h8)
+    assert dw.shape == (7, 40) and db.shape == (7,) and ops.ckpt8_decode(h8, torch.bfloat16).dtype == torch.bfloat16
+    t = m(32, 4, t=torch.float32)
+    assert ops.relpos_bias_1d(t, 3, 9, out_dtype=torch.float16).shape == (4, 3, 9) and ops.relpos_bias_1d(t, 3, 9, ld=12).shape == (4, 3, 12)
+    assert ops.relpos_bias_1d_backward(m(2, 4, 3, 9), 32).shape == (32, 4) and ops.swin_relpos_bias_backward(m(2, 4, 9, 9), 3).shape == (25, 4)
+
+
+@pytest.mark.parametrize("x", [lambda t: t(3, 1, 8).expand(3, 4, 8), lambda t: t(1, 4, 8).expand(3, 4, 8), lambda t: t(1, 8).expand(5, 8),
+                               lambda t: t(5, 16)[:, ::2], lambda t: t(8, 5).t(), lambda t: t(4, 3, 8).transpose(0, 1), lambda t: t(3, 6, 8)[:, :4],
+                               lambda t: t(5, 1).expand(5, 8), lambda t: t(1, 1).expand(5, 1), lambda t: t(40).as_strided((5, 8), (4, 1))])
+def test_rows_that_are_not_one_stride_apart_are_refused(x):
+    x = x(lambda *s: torch.empty(*s, device="meta"))
+    g = torch.empty(x.shape[-1], device="meta")
+    with pytest.raises(_lib.OvisError, match="one stride apart"):
+        ops.layernorm_forward(x, g, g)
+    with pytest.raises(_lib.OvisError, match="one stride apart"):
+        ops.act_forward_ckpt8(x, ops.ACT_RELU)
+
+
+@pytest.mark.parametrize("x", [lambda t: t(5, 24)[:, 8:16], lambda t: t(3, 4, 24)[..., :8], lambda t: t(9, 8)[::2], lambda t: t(3, 1, 24)[..., :8],
+                               lambda t: t(1, 8).expand(1, 8), lambda t: t(5, 3)[:, 1:2], lambda t: t(0, 8), lambda t: t(8)])
+def test_strided_rows_are_taken(x):
+    x = x(lambda *s: torch.empty(*s, device="meta"))
+    g = torch.empty(x.shape[-1], device="meta")
+    assert ops.layernorm_forward(x, g, g).y.shape == x.shape
+
+
+def test_no_autograd_graph_is_built():
+    m = lambda *s: torch.empty(*s, device="meta", requires_grad=True)
+    o = ops.layernorm_forward(m(5, 64), m(64), m(64), residual=m(5, 64), checkpoint=True)
+    outs = [o.y, o.sum, o.stats, *ops.layernorm_backward(m(5, 64), o.xhat8, o.stats, m(64)), *ops.linear_wgrad_ckpt8(m(5, 7), o.xhat8),
+            ops.act_forward_ckpt8(m(5, 64), ops.ACT_GELU)[0], ops.act_backward_ckpt8(m(5, 64), o.xhat8, ops.ACT_GELU)[0],
+            ops.relpos_bias_1d(m(32, 4), 3, 9), ops.relpos_bias_1d_backward(m(4, 3, 9), 32), ops.swin_relpos_bias_backward(m(4, 9, 9), 3)]
+    assert all(not t.requires_grad and t.grad_fn is None for t in outs)

@@ -364,7 +364,7 @@ extern "C" int ovis_layernorm_train_forward(const void* x, long long ldx, const 
                "layernorm_train_forward: y has x's type, or any where x is f32");
   const RowShape sh = row_shape(C, 4);
   const long long blocks = (rows + 256 / sh.lpr - 1) / (256 / sh.lpr);
-  OVIS_REQUIRE(blocks < (1ll << 31), "layernorm_train_forward: %lld rows are too many for one launch", rows);
+  OVIS_REQUIRE(blocks <= ovis::kMostBlocks, "layernorm_train_forward: %lld rows are too many for one launch", rows);
 #define LN_GO(TX, TY, LPR, NCH)                                                                                                             \
   hipLaunchKernelGGL((layernorm_train_fwd_kernel<TX, TY, LPR, NCH>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,            \
                      (const TX*)x, ldx, (const TX*)residual, ldr, gamma, beta, (TX*)sum, (TY*)y, stats, codes, scales, rows, C, eps)

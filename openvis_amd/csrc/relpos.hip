@@ -325,7 +325,7 @@ extern "C" int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, lon
   if (rc != OVIS_OK) return rc;
   const SeqShape s = seq_shape(B, H, Nq, Nk);
   const long long W = (long long)H * (Nq + Nk - 1);
-  OVIS_REQUIRE(s.lines <= 65535 && W < (1ll << 31), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
+  OVIS_REQUIRE(s.lines <= 65535 && s.strips <= ovis::kMostBlocks && W < (1ll << 31), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
 #define RP_LANES(T)                                                                                                                         \
   if (s.lanes == 64) { RP_GO(T, 64) } else if (s.lanes == 32) { RP_GO(T, 32) } else if (s.lanes == 16) { RP_GO(T, 16) } else { RP_GO(T, 8) }
 #define RP_GO(T, L)                                                                                                                         \

@@ -179,6 +179,9 @@ __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int n, u32x
 // sums the P lines of part [P][W] in a fixed order: columns below `split` to out0, the others to out1 (layernorm_train.hip)
 int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream);
 
+// a launch's lanes along a dimension are counted in 32 bits: so many workgroups of 256 lanes at most
+constexpr long long kMostBlocks = (1ll << 24) - 1;
+
 inline bool dtype_ok(int t) { return t == OVIS_F32 || t == OVIS_F16 || t == OVIS_BF16; }
 inline int dtype_size(int t) { return t == OVIS_F32 ? 4 : 2; }
 

@@ -502,7 +502,7 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
                K, lddy, dtype);
   const WgradShape w = wgrad_shape(M, N, K, dtype);
   const long long blocks = (long long)w.tiles_n * w.tiles_k * w.S;
-  OVIS_REQUIRE(blocks < (1ll << 31) && lddy < (1ll << 24) && K < (1 << 24), "linear_wgrad_ckpt8: %d x %d (row stride %lld) is too large for one call", N,
+  OVIS_REQUIRE(blocks <= ovis::kMostBlocks && (long long)N * K < (1ll << 34) && lddy < (1ll << 24) && K < (1 << 24), "linear_wgrad_ckpt8: %d x %d (row stride %lld) is too large for one call", N,
                K, lddy);
   const bool join = w.S > 1 || gamma;
   float* part = join ? workspace : dw;

@@ -91,6 +91,15 @@ def test_weight_gradient_entry_point_refuses():
     assert "too large" in change(a1=1 << 24) and "too large" in change(a11=1 << 24)
 
 
+def test_launches_of_2_to_the_32_lanes_are_refused():
+    """all of these fit in the card's memory, but not in one launch"""
+    assert "too many for one launch" in _refused("ovis_layernorm_train_forward", "plplppppppplifiip", P, 2056, None, 0, P, P, None, P, P, None, None, 1 << 24, 2056,
+                                                 1e-5, 1, 1, None)
+    b = (ctypes.c_int * 3)(1, 2, 4)
+    assert "too large" in _refused("ovis_relpos_bias_1d_backward", "plllpppiiliiilip", P, 0, 0, 1, P, P, b, 3, 1, 1, 1, (1 << 30) - 1, 66, 0, 1, None)
+    assert "too large" in _refused("ovis_linear_wgrad_ckpt8", "plpppppppliiip", P, 1 << 20, P, P, None, None, P, P, P, 1, 1 << 20, 1 << 20, 1, None)
+
+
 def test_tensors_on_the_host_are_refused():
     x, g = torch.zeros(4, 64), torch.ones(64)
     ck = ops.Ckpt8(torch.zeros(4, 64).to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8).view(torch.float8_e8m0fnu))

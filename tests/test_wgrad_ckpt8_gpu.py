@@ -136,12 +136,13 @@ def test_strided_rows_no_rows(dt):
     assert dw.shape == (5, 40) and not dw.any() and not db.any()
 
 
-def test_same_bits_on_another_stream_and_in_a_replayed_graph():
+@pytest.mark.parametrize("M,N,K", [(9000, 300, 520), (9000, 2048, 2100)])       # the second: the largest tile, the scales' maxima beforehand
+def test_same_bits_on_another_stream_and_in_a_replayed_graph(M, N, K):
     from openvis_amd import ops
     g = torch.Generator().manual_seed(1)
-    dy = torch.randn(9000, 300, generator=g).half().cuda()
-    x8 = ops.ckpt8_encode(torch.randn(9000, 520, generator=g).cuda())
-    gamma, beta = torch.randn(520, generator=g).cuda(), torch.randn(520, generator=g).cuda()
+    dy = torch.randn(M, N, generator=g).half().cuda()
+    x8 = ops.ckpt8_encode(torch.randn(M, K, generator=g).cuda())
+    gamma, beta = torch.randn(K, generator=g).cuda(), torch.randn(K, generator=g).cuda()
 
     def step():
         return ops.linear_wgrad_ckpt8(dy, x8, gamma=gamma, beta=beta)

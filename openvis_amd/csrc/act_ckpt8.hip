@@ -62,14 +62,14 @@ __device__ __forceinline__ void activation(float h, float& y, float& slope) {
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256)
 act_ckpt8_fwd_kernel(const T* __restrict__ h, long long ldh, T* __restrict__ y, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                     unsigned slots, unsigned per_row, int C) {
+                     unsigned slots, unsigned per_row, long long rows, int C) {
   const unsigned i = blockIdx.x * 256u + threadIdx.x;
   if (i >= slots) return;                                        // slots is a multiple of 4: a block's lanes leave together
   const unsigned row = i / per_row, v = i - row * per_row;
   const int col = (int)v * 8, n = C - col;
   float x[8];
   if (n > 0) {
-    load8(h + (long long)row * ldh + col, n, x);
+    load8(h + (long long)row * ldh + col, n, (long long)row + 8 < rows, x);          // eight rows on, a row's end is not the tensor's
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.f;
@@ -207,7 +207,7 @@ extern "C" int ovis_act_ckpt8_forward(const void* h, long long ldh, void* y, uin
   const unsigned slots = (unsigned)(rows * per_row);
 #define ACT_GO(T, A)                                                                                                                        \
   hipLaunchKernelGGL((act_ckpt8_fwd_kernel<T, A>), dim3(ovis::cdiv(slots, 256)), dim3(256), 0, (hipStream_t)stream, (const T*)h, ldh,      \
-                     (T*)y, codes, scales, slots, (unsigned)per_row, C)
+                     (T*)y, codes, scales, slots, (unsigned)per_row, rows, C)
 #define ACT_ALL(T) switch (act) { case 0: ACT_GO(T, 0); break; case 1: ACT_GO(T, 1); break; case 2: ACT_GO(T, 2); break; default: ACT_GO(T, 3); }
   ACT_TYPE(dtype, ACT_ALL)
 #undef ACT_GO

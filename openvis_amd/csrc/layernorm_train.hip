@@ -40,16 +40,17 @@ layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __
   const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const bool live = row < rows;                                  // lanes of a row behind the last one stay for the shuffles
   const long long r = live ? row : rows - 1;
+  const bool on = row + 8 < rows;                                // eight rows on, a row's end is not the tensor's
   float v[NCH][8];
   float s = 0.f;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int col = (c * LPR + li) * 8, n = C - col;
     if (n > 0) {
-      load8(x + r * ldx + col, n, v[c]);
+      load8(x + r * ldx + col, n, on, v[c]);
       if (res) {
         float t[8];
-        load8(res + r * ldr + col, n, t);
+        load8(res + r * ldr + col, n, on, t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[c][e] = (float)(TX)(v[c][e] + t[e]);
         if (live) store8(sum + r * C + col, n, v[c]);

@@ -23,7 +23,8 @@ template <> struct Vec8Of<__bf16> { using type = bf16x8_u; };
 template <> struct Vec8Of<float> { using type = f32x8_u; };
 typedef unsigned u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
 
-// n (1..8) elements of p into v, the others 0
+// n (1..8) elements of p into v, the others 0.  Here and below a row's last elements are read at indexes held at n - 1, without conditions, so that
+// the reads are in flight together: one condition each makes the compiler wait for each.
 template <typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)[8]) {
   if (n >= 8) {
@@ -32,8 +33,18 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int n, float (&v)
     for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < n ? (float)p[e] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = (float)p[e < n ? e : n - 1];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
   }
+}
+
+// the same where `on` says that eight elements can be read: what follows a row's end is the next rows', and becomes 0
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ p, int n, bool on, float (&v)[8]) {
+  load8(p, on ? 8 : n, v);
+#pragma unroll
+  for (int e = 1; e < 8; ++e) v[e] = e < n ? v[e] : 0.f;
 }
 
 // the same, kept in the stored type
@@ -48,9 +59,11 @@ struct Raw8 {
       if (n >= 8 || on) {
         v = *reinterpret_cast<const typename Vec8Of<T>::type*>(p);
       } else {
+        T t[7];
 #pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (e < n) v[e] = p[e];
+        for (int e = 0; e < 7; ++e) t[e] = p[e < n ? e : n - 1];
+#pragma unroll
+        for (int e = 0; e < 7; ++e) v[e] = t[e];
       }
     }
   }
@@ -156,9 +169,13 @@ __device__ __forceinline__ u32x2_u load_codes(const uint8_t* __restrict__ p, int
     c = *reinterpret_cast<const u32x2_u*>(p);
   } else {
     c[0] = c[1] = 0u;
+    if (n > 0) {
+      unsigned t[7];
 #pragma unroll
-    for (int e = 0; e < 7; ++e)
-      if (e < n) c[e >> 2] |= (unsigned)p[e] << (8 * (e & 3));
+      for (int e = 0; e < 7; ++e) t[e] = p[e < n ? e : n - 1];
+#pragma unroll
+      for (int e = 0; e < 7; ++e) c[e >> 2] |= e < n ? t[e] << (8 * (e & 3)) : 0u;
+    }
   }
   return c;
 }

@@ -53,12 +53,16 @@ __device__ __forceinline__ int at(int m, int c) {
 
 template <typename T> struct DyOf {                              // 8 elements of dY as loaded
   u16x8 v;
-  __device__ __forceinline__ void load(const T* p, int n) {
+  __device__ __forceinline__ void load(const T* p, int n) {      // n <= 0: none
+    v = (u16x8)0;
     if (n >= 8) {
       load_all(p);
-    } else {
+    } else if (n > 0) {
+      T t[7];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? __builtin_bit_cast(unsigned short, p[e]) : (unsigned short)0;
+      for (int e = 0; e < 7; ++e) t[e] = p[e < n ? e : n - 1];
+#pragma unroll
+      for (int e = 0; e < 7; ++e) v[e] = e < n ? __builtin_bit_cast(unsigned short, t[e]) : (unsigned short)0;
     }
   }
   __device__ __forceinline__ void load_all(const T* p) { v = __builtin_bit_cast(u16x8, *reinterpret_cast<const typename Vec8Of<T>::type*>(p)); }
@@ -67,7 +71,11 @@ template <typename T> struct DyOf {                              // 8 elements o
 };
 template <> struct DyOf<float> {
   float v[8];
-  __device__ __forceinline__ void load(const float* p, int n) { load8(p, n, v); }
+  __device__ __forceinline__ void load(const float* p, int n) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (n > 0) load8(p, n, v);
+  }
   __device__ __forceinline__ void load_all(const float* p) { load8(p, 8, v); }
   __device__ __forceinline__ float value(int e) const { return v[e]; }
   __device__ __forceinline__ u16x8 plane(int i) const {         // the i-th bf16 term of v (each the rest rounded to nearest)

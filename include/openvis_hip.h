@@ -604,7 +604,7 @@ int ovis_ckpt8_decode(const uint8_t* codes, const uint8_t* scales, void* out, lo
  *   workspaces of the ..._workspace_bytes. */
 int ovis_relpos_bias_1d(const float* table, void* out, const int* borders_host, int nborders, int bidirectional, int H, int Nq, int Nk, int ld,
                         long long q_offset, int dtype, ovis_stream_t stream);
-long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk);
+long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk, int buckets);
 int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace,
                                  const int* borders_host, int nborders, int bidirectional, long long B, int H, int Nq, int Nk,
                                  long long q_offset, int dtype, ovis_stream_t stream);

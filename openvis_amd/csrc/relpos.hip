@@ -27,6 +27,16 @@ __device__ __forceinline__ int bucket_of(long long r, const int* at, int n, int 
   return lo + (both && r > 0 ? n + 1 : 0);
 }
 
+// the bucket's r = j - i - off, as a run [r0, r1)
+__device__ __forceinline__ void bucket_run(int bk, const int* at, int n, int both, long long& r0, long long& r1) {
+  const int side = n + 1;
+  const bool pos = both && bk >= side;
+  const int k = pos ? bk - side : bk;
+  const long long far = 1ll << 61, first = k == 0 ? 0 : at[k - 1], last = k == n ? far : at[k];      // magnitudes [first, last)
+  r0 = pos ? (first > 1 ? first : 1) : 1 - last;
+  r1 = pos ? last : k == 0 && !both ? far : 1 - first;                                                     // one direction: r > 0 is distance 0 too
+}
+
 // A workgroup writes 256 V columns (V = 16 bytes) of a run of rows of one head.  Row i + 1 is row i moved one column on, so the values of all
 // its diagonals are laid out once in LDS and a lane holds its V columns in registers, takes one new value a row and moves the others on.
 template <typename T>
@@ -67,19 +77,26 @@ relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders 
   }
 }
 
+// Rows of a lane that are fetched at once: eight (8 x 8 x 1023^2 bf16 37 us, by fours 40 us); four where rows are so short that most of eight
+// would lie outside (9 x 20 x 3834 x 32 f32 34 us, by eights 42 us).
+constexpr int rows_in_flight(int lanes) { return lanes == 8 ? 4 : 8; }
+
 // Diagonal sums.  A wavefront owns 64 V diagonals, V neighbouring ones a lane, and walks down the rows of its share: the lane's V elements
 // of the next row lie one element on, so they are loaded as one vector at any element's address and added to the same registers -- no
 // transposition, no LDS, no atomics.  Where a row is short, L < 64 lanes take 8 L diagonals and 64 / L rows go at once: a strip of 8 L diagonals
-// meets rows of Nk columns, so 8 L beyond Nk is idle (9 x 20 x 3834 x 32 f32: 102 us with 64 lanes).  A vector that crosses an end of its row is read all the same, from the neighbouring rows' elements, and
-// masked; only where it would leave the tensor's span (first and last rows) are its elements read one by one: a separate read of a row's ends
+// meets rows of Nk columns, so 8 L beyond Nk is idle (9 x 20 x 3834 x 32 f32: 102 us with 64 lanes).  A vector that crosses an end of its row is read all the
+// same, from the neighbouring rows' elements, and masked; only where it would leave the tensor's span (first and last rows) are its elements read one by one: a separate read of a row's ends
 // cost more than the rows themselves (8 x 8 x 1023^2 bf16: 50 us).  A workgroup is four wavefronts on the same diagonals, rows dealt in turn;
-// its sums are one line of the workspace.  grid: (diagonal strips, row chunks x batch, heads).
+// it adds its diagonals up by buckets, 16 lanes a bucket, into one line of the workspace [buckets][H] (a line of diagonals and a launch that
+// sums them afterwards: 4 to 5 us more).  grid: (diagonal strips, row chunks x batch, heads).
 template <typename T, int L>
 __global__ void __launch_bounds__(256)
-relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, long long B, int bper, int Nq,
-                  int Nk, int rows, int chunks) {
-  constexpr int V = 8, U = 4, RG = 256 / L;                      // U rows in flight, RG row groups
+relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, Borders borders, int both,
+                  long long off, long long B, long long bper, int Nq, int Nk, int rows, int chunks) {
+  constexpr int V = 8, U = rows_in_flight(L), RG = 256 / L;      // RG row groups
   __shared__ float buf[RG][L * V + 4];
+  __shared__ int edge[kMaxBuckets];                              // the borders: searched at the end, read from the arguments' memory (slow) at once
+  const int mine = (int)threadIdx.x < borders.n ? borders.at[threadIdx.x] : 0;
   const int lane = threadIdx.x % L;
   const int grp = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : threadIdx.x / L;
   const int h = blockIdx.z, ck = blockIdx.y % chunks;
@@ -136,45 +153,28 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
   }
 #pragma unroll
   for (int e = 0; e < V; ++e) buf[grp][lane * V + e] = acc[e];
+  edge[threadIdx.x] = mine;
   __syncthreads();
-  float* line = part + ((long long)blockIdx.y * gridDim.z + h) * D;
-  for (int k = threadIdx.x; k < L * V; k += 256)
-    if (d0 + k < D) {
-      float t = buf[0][k];
+  for (int k = threadIdx.x; k < L * V; k += 256) {
+    float t = buf[0][k];
 #pragma unroll
-      for (int w = 1; w < RG; ++w) t += buf[w][k];
-      line[d0 + k] = t;
-    }
-}
-
-// sum over a workgroup's 256 values, in a fixed order
-__device__ __forceinline__ float block_sum(float s, float* buf) {
-  buf[threadIdx.x] = s;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o) buf[threadIdx.x] += buf[threadIdx.x + o];
-    __syncthreads();
+    for (int w = 1; w < RG; ++w) t += buf[w][k];
+    buf[0][k] = t;
   }
-  return buf[0];
-}
-
-// dtable[bucket, h]: the sum over the bucket's run of diagonals
-__global__ void __launch_bounds__(256)
-relpos_bwd_finish_kernel(const float* __restrict__ diag, float* __restrict__ dtable, Borders b, int both, int H, int Nq, int Nk, long long off) {
-  __shared__ float buf[256];
-  const int bk = blockIdx.x, h = blockIdx.y, D = Nq + Nk - 1, side = b.n + 1;
-  // the bucket's r = j - i - off, as a run [r0, r1)
-  const bool pos = both && bk >= side;
-  const int k = pos ? bk - side : bk;
-  const long long far = 1ll << 61, first = k == 0 ? 0 : b.at[k - 1], last = k == b.n ? far : b.at[k];      // magnitudes [first, last)
-  const long long r0 = pos ? (first > 1 ? first : 1) : 1 - last;
-  const long long r1 = pos ? last : k == 0 && !both ? far : 1 - first;                                     // one direction: r > 0 is distance 0 too
-  const long long shift = (long long)(Nq - 1) + off;
-  const long long d0 = min(max(r0 + shift, 0ll), (long long)D), d1 = min(max(r1 + shift, 0ll), (long long)D);
-  float s = 0.f;
-  for (long long d = d0 + threadIdx.x; d < d1; d += 256) s += diag[(long long)h * D + d];
-  s = block_sum(s, buf);
-  if (threadIdx.x == 0) dtable[(long long)bk * H + h] = s;
+  __syncthreads();
+  const int buckets = (borders.n + 1) * (both ? 2 : 1), end = D - d0 < L * V ? D - d0 : L * V;
+  float* line = part + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * buckets * gridDim.z + h;
+  for (int bk = threadIdx.x >> 4; bk < buckets; bk += 16) {
+    long long r0, r1;
+    bucket_run(bk, edge, borders.n, both, r0, r1);
+    const long long shift = (long long)(Nq - 1) + off - d0;      // r = j - i - off lies on the strip's diagonal r + shift
+    const int k0 = (int)min(max(r0 + shift, 0ll), (long long)end), k1 = (int)min(max(r1 + shift, 0ll), (long long)end);
+    float t = 0.f;
+    for (int k = k0 + (threadIdx.x & 15); k < k1; k += 16) t += buf[0][k];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) t += __shfl_xor(t, o, 16);
+    if ((threadIdx.x & 15) == 0) line[(long long)bk * gridDim.z] = t;
+  }
 }
 
 // Windows: sum over a run of the batch, element by element (grid: pieces of the [H, N, N] plane, batch chunks), then over the pairs of each
@@ -239,19 +239,25 @@ window_bias_finish_kernel(const float* __restrict__ sum, float* __restrict__ dta
   }
 }
 
-// Workgroups: about sixteen a CU; a long sequence's rows are split, a large batch's entries go several to one.
-struct SeqShape { int lanes, strips, chunks, rows, bper; long long lines; };
+// Workgroups: about ten a CU (8 x 8 x 1023^2 bf16 34.5 us; six 41, sixteen 36.5; 16384^2 fp16 124, 154, 132); a long sequence's rows are split, a large batch's entries go several to one.
+// Few rows and entries: one workgroup a head takes them all, and no second launch adds up lines (4 x 6 x 47 x 47: 10 us in two launches).
+struct SeqShape { int lanes, strips, chunks, rows; long long bper, lines; };
 inline SeqShape seq_shape(long long B, int H, int Nq, int Nk) {
   SeqShape s;
+  for (int lanes = 8; lanes <= 64; lanes *= 2) {
+    const int pass = rows_in_flight(lanes) * (256 / lanes);
+    if ((long long)Nq + Nk - 1 <= 8 * lanes && B * ((Nq + pass - 1) / pass) <= 6) return {lanes, 1, 1, Nq, B, 1};
+  }
   s.lanes = Nk >= 512 ? 64 : Nk >= 256 ? 32 : Nk >= 128 ? 16 : 8;
   s.strips = (int)(((long long)Nq + Nk - 1 + 8 * s.lanes - 1) / (8 * s.lanes));
   const long long per = B * H * s.strips;
-  long long want = (4096 + per - 1) / per;
+  long long want = (2560 + per - 1) / per;
   const long long most = (Nq + 2048 / s.lanes - 1) / (2048 / s.lanes);              // eight passes of rows at least
   if (want > most) want = most;
-  s.rows = (int)((Nq + want - 1) / want);
+  const int pass = rows_in_flight(s.lanes) * (256 / s.lanes);
+  s.rows = ((int)((Nq + want - 1) / want) + pass - 1) / pass * pass;               // whole passes
   s.chunks = (Nq + s.rows - 1) / s.rows;
-  s.bper = (int)(per > 4096 ? (per + 4095) / 4096 : 1);
+  s.bper = per > 2560 ? (per + 2559) / 2560 : 1;
   s.lines = (B + s.bper - 1) / s.bper * s.chunks;
   return s;
 }
@@ -308,9 +314,10 @@ extern "C" int ovis_relpos_bias_1d(const float* table, void* out, const int* bor
   return ovis::check_launch("relpos_bias_1d");
 }
 
-extern "C" long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk) {
-  if (B <= 0 || H <= 0 || Nq <= 0 || Nk <= 0) return 0;
-  return (seq_shape(B, H, Nq, Nk).lines + 1) * H * ((long long)Nq + Nk - 1) * 4;
+extern "C" long long ovis_relpos_bias_1d_backward_workspace_bytes(long long B, int H, int Nq, int Nk, int buckets) {
+  if (B <= 0 || H <= 0 || Nq <= 0 || Nk <= 0 || buckets <= 0) return 0;
+  const SeqShape s = seq_shape(B, H, Nq, Nk);
+  return s.lines * s.strips * H * buckets * 4;
 }
 
 extern "C" int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, long long hs, long long ld, float* dtable, float* workspace,
@@ -324,24 +331,22 @@ extern "C" int ovis_relpos_bias_1d_backward(const void* dbias, long long bs, lon
   const int rc = fill_borders(b, borders_host, nborders);
   if (rc != OVIS_OK) return rc;
   const SeqShape s = seq_shape(B, H, Nq, Nk);
-  const long long W = (long long)H * (Nq + Nk - 1);
-  OVIS_REQUIRE(s.lines <= 65535 && s.strips <= ovis::kMostBlocks && W < (1ll << 31), "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
+  const int buckets = (b.n + 1) * (bidirectional ? 2 : 1), W = buckets * H;                               // at most 514 x 65535
+  const long long parts = s.lines * s.strips;
+  OVIS_REQUIRE(s.lines <= 65535 && s.strips <= ovis::kMostBlocks && parts < (1ll << 31) && (long long)H * (Nq + Nk - 1) < (1ll << 31),
+               "relpos_bias_1d_backward: B %lld, H %d, Nq %d, Nk %d are too large for one call", B, H, Nq, Nk);
+  float* to = parts > 1 ? workspace : dtable;
 #define RP_LANES(T)                                                                                                                         \
   if (s.lanes == 64) { RP_GO(T, 64) } else if (s.lanes == 32) { RP_GO(T, 32) } else if (s.lanes == 16) { RP_GO(T, 16) } else { RP_GO(T, 8) }
 #define RP_GO(T, L)                                                                                                                         \
   hipLaunchKernelGGL((relpos_bwd_kernel<T, L>), dim3(s.strips, (unsigned)s.lines, H), dim3(256), 0, (hipStream_t)stream, (const T*)dbias, bs,  \
-                     hs, ld, workspace + W, B, s.bper, Nq, Nk, s.rows, s.chunks);
+                     hs, ld, to, b, bidirectional, q_offset, B, s.bper, Nq, Nk, s.rows, s.chunks);
   RP_TYPE(dtype, RP_LANES)
 #undef RP_LANES
 #undef RP_GO
-  int rc2 = ovis::check_launch("relpos_bias_1d_backward");
-  if (rc2 == OVIS_OK && s.lines > 1)
-    rc2 = ovis::column_sum_finish(workspace + W, (int)s.lines, (int)W, workspace, (int)W, workspace, (hipStream_t)stream);
-  if (rc2 != OVIS_OK) return rc2;
-  const int buckets = (b.n + 1) * (bidirectional ? 2 : 1);
-  hipLaunchKernelGGL(relpos_bwd_finish_kernel, dim3(buckets, H), dim3(256), 0, (hipStream_t)stream, s.lines > 1 ? workspace : workspace + W,
-                     dtable, b, bidirectional, H, Nq, Nk, q_offset);
-  return ovis::check_launch("relpos_bias_1d_backward");
+  const int launched = ovis::check_launch("relpos_bias_1d_backward");
+  if (launched != OVIS_OK || parts == 1) return launched;
+  return ovis::column_sum_finish(workspace, (int)parts, W, dtable, W, dtable, (hipStream_t)stream);
 }
 
 extern "C" long long ovis_swin_relpos_bias_backward_workspace_bytes(long long B, int H, int ws) {

@@ -277,7 +277,7 @@ Tensor relpos_bias_1d_backward(const Tensor& dbias, const Tensor& borders, bool 
   Tensor out = at::empty({buckets, g.H}, o);
   if (!on.meta) {
     const int H = small(name, g.H), Nq = small(name, g.Nq), Nk = small(name, g.Nk);
-    Tensor ws = words(dbias, ovis_relpos_bias_1d_backward_workspace_bytes(g.B, H, Nq, Nk));
+    Tensor ws = words(dbias, ovis_relpos_bias_1d_backward_workspace_bytes(g.B, H, Nq, Nk, (int)buckets));
     done(name, ovis_relpos_bias_1d_backward(dbias.const_data_ptr(), g.bs, g.hs, g.ld, out.data_ptr<float>(), ws.data_ptr<float>(), borders.const_data_ptr<int>(),
                                             nb, both, g.B, H, Nq, Nk, q_offset, d, cur_stream()));
   }

@@ -17,17 +17,42 @@ namespace {
 
 using namespace ovis;
 
-// sum over the LPR lanes of a row; LPR = 256 crosses the four wavefronts through `buf` (two alternating slots, so that one barrier is enough)
-template <int LPR>
-__device__ __forceinline__ float row_sum(float v, float* buf) {
+// sums over the LPR lanes of a row, N of them side by side: moves between lanes of the vector unit, no LDS (by LDS permutes a step takes ten times
+// as long, and a row's sums are a chain of them).  LPR = 256 crosses the four wavefronts through `buf`, with one barrier: the caller alternates
+// between two of them.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int LPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (&buf)[N][4]) {
 #pragma unroll
-  for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  if constexpr (LPR > 64) {
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+  for (int i = 0; i < N; ++i) {
+    float t = v[i];
+    t = dpp_add<0xB1>(t);                                        // lanes 1 0 3 2 of four
+    t = dpp_add<0x4E>(t);                                        // lanes 2 3 0 1
+    t = dpp_add<0x141>(t);                                       // mirrored within eight: the other four
+    t = dpp_add<0x140>(t);                                       // mirrored within sixteen: the other eight
+    if constexpr (LPR >= 32) {
+      const unsigned u = __builtin_bit_cast(unsigned, t);
+      const auto w = __builtin_amdgcn_permlane16_swap(u, u, false, false);         // the even and the odd sixteens
+      t = __builtin_bit_cast(float, (unsigned)w[0]) + __builtin_bit_cast(float, (unsigned)w[1]);
+    }
+    if constexpr (LPR >= 64) {
+      const unsigned u = __builtin_bit_cast(unsigned, t);
+      const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      t = __builtin_bit_cast(float, (unsigned)w[0]) + __builtin_bit_cast(float, (unsigned)w[1]);
+    }
+    v[i] = t;
   }
-  return v;
+  if constexpr (LPR > 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((threadIdx.x & 63) == 0) buf[i][threadIdx.x >> 6] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (buf[i][0] + buf[i][1]) + (buf[i][2] + buf[i][3]);
+  }
 }
 
 template <typename TX, typename TY, int LPR, int NCH>
@@ -35,14 +60,14 @@ __global__ void __launch_bounds__(256)
 layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __restrict__ res, long long ldr, const float* __restrict__ gamma,
                            const float* __restrict__ beta, TX* __restrict__ sum, TY* __restrict__ y, float* __restrict__ stats,
                            uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, long long rows, int C, float eps) {
-  __shared__ float buf[2][4];
+  __shared__ float buf[2][1][4];
   const int li = threadIdx.x % LPR;
   const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   const bool live = row < rows;                                  // lanes of a row behind the last one stay for the shuffles
   const long long r = live ? row : rows - 1;
   const bool on = row + 8 < rows;                                // eight rows on, a row's end is not the tensor's
   float v[NCH][8];
-  float s = 0.f;
+  float s[1] = {0.f}, q[1] = {0.f};
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int col = (c * LPR + li) * 8, n = C - col;
@@ -60,20 +85,21 @@ layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __
       for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += v[c][e];
+    for (int e = 0; e < 8; ++e) s[0] += v[c][e];
   }
-  const float mean = row_sum<LPR>(s, buf[0]) / (float)C;
-  float q = 0.f;
+  row_sums<LPR>(s, buf[0]);
+  const float mean = s[0] / (float)C;
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int n = C - (c * LPR + li) * 8;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       v[c][e] = e < n ? v[c][e] - mean : 0.f;
-      q += v[c][e] * v[c][e];
+      q[0] += v[c][e] * v[c][e];
     }
   }
-  const float rstd = 1.f / sqrtf(row_sum<LPR>(q, buf[1]) / (float)C + eps);
+  row_sums<LPR>(q, buf[1]);
+  const float rstd = 1.f / sqrtf(q[0] / (float)C + eps);
   if (live && li == 0) {
     stats[2 * r] = mean;
     stats[2 * r + 1] = rstd;
@@ -113,7 +139,7 @@ __global__ void __launch_bounds__(256, WAVES)
 layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
                            const uint8_t* __restrict__ scales, const float* __restrict__ stats, const float* __restrict__ gamma,
                            const TX* __restrict__ dsum, long long ldds, TX* __restrict__ dx, float* __restrict__ part, long long rows, int C) {
-  __shared__ float buf[4][4];
+  __shared__ float buf[2][2][4];
   extern __shared__ float acc[];                                 // [2][Cp]: gamma in the first line, at the end the workgroup's sums
   const int li = threadIdx.x % LPR, Cp = NCH * LPR * 8;
   constexpr int RPB = 256 / LPR;
@@ -178,7 +204,7 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
         for (int e = 0; e < 8; ++e) v[e] = e < n ? (h[c].at(e) - mean) * rstd : 0.f;
       }
     };
-    float s1 = 0.f, s2 = 0.f;
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const float* g = acc + (c * LPR + li) * 8;
@@ -189,14 +215,14 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
       for (int e = 0; e < 8; ++e) {
         if constexpr (TAIL && CK) v[e] = e < n ? v[e] : 0.f;     // without codes xhat has done so
         const float de = TAIL && e >= n ? 0.f : d[c].at(e), gd = de * g[e];
-        s1 += gd;
-        s2 += gd * v[e];
+        s[0] += gd;
+        s[1] += gd * v[e];
         dg[c][e] += de * v[e];
         db[c][e] += de;
       }
     }
-    const float c1 = row_sum<LPR>(s1, buf[2 * phase]) / (float)C;
-    const float c2 = row_sum<LPR>(s2, buf[2 * phase + 1]) / (float)C;
+    row_sums<LPR>(s, buf[phase]);
+    const float c1 = s[0] / (float)C, c2 = s[1] / (float)C;
     phase ^= 1;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {                              // from here on the stored forms are widened again, not kept widened

@@ -51,7 +51,10 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (&buf)[N][4]) {
       if ((threadIdx.x & 63) == 0) buf[i][threadIdx.x >> 6] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = (buf[i][0] + buf[i][1]) + (buf[i][2] + buf[i][3]);
+    for (int i = 0; i < N; ++i) {
+      if constexpr (LPR == 128) v[i] = threadIdx.x < 128 ? buf[i][0] + buf[i][1] : buf[i][2] + buf[i][3];
+      else v[i] = (buf[i][0] + buf[i][1]) + (buf[i][2] + buf[i][3]);
+    }
   }
 }
 
@@ -269,22 +272,25 @@ layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* 
 
 struct RowShape { int lpr, nch; };
 // Lanes per row: the fewest that hold the row in `most` pieces each, since a lane's extra pieces are loads in flight while a lane behind the
-// row's end is idle.
+// row's end is idle.  128 lanes in two pieces are no gain over 256 in one for 16-bit rows (27286 x 1800 backward 83 us against 78; 27286 x 3000 in
+// three pieces 119 us, by 256 lanes in two 179 us; f32 of 1600 columns 62 us against 70).
 inline RowShape row_shape(int C, int most) {
   const int nvec = (C + 7) / 8;
-  for (int lpr : {16, 32, 64, 256})
-    if ((nvec + lpr - 1) / lpr <= most) return {lpr, (nvec + lpr - 1) / lpr};
+  for (int lpr : {16, 32, 64, 128, 256}) {
+    const int nch = (nvec + lpr - 1) / lpr;
+    if (nch <= most && !(most == 3 && lpr == 128 && nch < 3)) return {lpr, nch};
+  }
   return {256, (nvec + 255) / 256};                              // C <= 8192: at most four
 }
 // Backward: a piece is 16 sums and two rows' dy, x and dsum: three pieces of 16-bit rows (220 registers) or two of f32 rows (192), two
-// wavefronts a SIMD.  98500 x 768 fp16 in three pieces 133 us, in two 144 us; 73600 x 384 f32 in three 87 us, in two 83 us (before the fetch
+// wavefronts a SIMD; two pieces of 16-bit rows (165), three wavefronts (27286 x 4096: 147 us, with two wavefronts 169 us).  98500 x 768 fp16 in three pieces 133 us, in two 144 us; 73600 x 384 f32 in three 87 us, in two 83 us (before the fetch
 // ahead).  Rows of more than 4096 f32 or 6144 16-bit columns need more and spill.
 inline RowShape bwd_row_shape(int C, int x_dtype) { return row_shape(C, x_dtype == OVIS_F32 ? 2 : 3); }
 
 // as many workgroups as the card holds at once: each walks over its rows, and a workgroup that had to wait would walk alone at the end
-constexpr int bwd_waves(int nch) { return nch == 1 ? 4 : 2; }
-inline unsigned bwd_blocks(long long rows, const RowShape& s) {
-  const long long need = (rows + 256 / s.lpr - 1) / (256 / s.lpr), full = 256 * bwd_waves(s.nch);
+constexpr int bwd_waves(int nch, bool f32) { return nch == 1 ? 4 : nch == 2 && !f32 ? 3 : 2; }
+inline unsigned bwd_blocks(long long rows, const RowShape& s, int x_dtype) {
+  const long long need = (rows + 256 / s.lpr - 1) / (256 / s.lpr), full = 256 * bwd_waves(s.nch, x_dtype == OVIS_F32);
   if (need <= 4) return 1;                                       // and no second launch: the workgroup's sums are the gradients
   const long long most = rows / 10 < 256 ? 256 : rows / 10 < full ? rows / 10 : full;    // a workgroup's line of sums costs as much as three rows
   return (unsigned)(need < most ? need : most);
@@ -299,10 +305,13 @@ namespace ovis {
 // many workgroups.  wide: a lane takes four columns and all lines.  The wide form needs no exchange but fills the card only from
 // tens of thousands of columns on: 33 lines of 124416 columns 5 us against 20, 126 lines of 29282 columns 40 us against 6.
 __global__ void __launch_bounds__(1024)
-column_sum_narrow_kernel(const float* __restrict__ part, int P, int W, float* __restrict__ out0, int split, float* __restrict__ out1) {
+column_sum_narrow_kernel(ColumnSum a, ColumnSum b, unsigned first) {             // workgroups from `first` on: b
   __shared__ float buf[64][17];
+  const ColumnSum& k = blockIdx.x < first ? a : b;
+  const float* part = k.part;
+  const int P = k.P, W = k.W;
   const int c = threadIdx.x & 15, p0 = threadIdx.x >> 4;
-  const int w = blockIdx.x * 16 + c;
+  const int w = (blockIdx.x - (blockIdx.x < first ? 0 : first)) * 16 + c;
   float s = 0.f;
   if (w < W)
     for (int p = p0; p < P; p += 64) s += part[(long long)p * W + w];
@@ -313,8 +322,8 @@ column_sum_narrow_kernel(const float* __restrict__ part, int P, int W, float* __
     __syncthreads();
   }
   if (p0 == 0 && w < W) {
-    if (w < split) out0[w] = buf[0][c];
-    else out1[w - split] = buf[0][c];
+    if (w < k.split) k.out0[w] = buf[0][c];
+    else k.out1[w - k.split] = buf[0][c];
   }
 }
 
@@ -351,8 +360,14 @@ int column_sum_finish(const float* part, int P, int W, float* out0, int split, f
   if (W >= 65536)
     hipLaunchKernelGGL(column_sum_wide_kernel, dim3(cdiv(W, 1024)), dim3(256), 0, stream, part, P, W, out0, split, out1);
   else
-    hipLaunchKernelGGL(column_sum_narrow_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, part, P, W, out0, split, out1);
+    hipLaunchKernelGGL(column_sum_narrow_kernel, dim3(cdiv(W, 16)), dim3(1024), 0, stream, ColumnSum{part, P, W, out0, split, out1}, ColumnSum{}, cdiv(W, 16));
   return check_launch("column_sum_finish");
+}
+
+int column_sum_two(const ColumnSum& a, const ColumnSum& b, hipStream_t stream) {
+  const unsigned first = cdiv(a.W, 16);
+  hipLaunchKernelGGL(column_sum_narrow_kernel, dim3(first + cdiv(b.W, 16)), dim3(1024), 0, stream, a, b, first);
+  return check_launch("column_sum_two");
 }
 
 }  // namespace ovis
@@ -369,17 +384,18 @@ int column_sum_finish(const float* part, int P, int W, float* out0, int split, f
     default: return ovis::fail(OVIS_EINVAL, "layernorm_train: no kernel for rows of %d", C);        \
   }
 #define LN_CASE(TX, TY, LPR, NCH) case LPR * 8 + NCH: LN_GO(TX, TY, LPR, NCH); break;
-#define LN_WIDE(TX, TY) LN_CASE(TX, TY, 256, 2) LN_CASE(TX, TY, 256, 3) LN_CASE(TX, TY, 256, 4)
 // the shapes that row_shape(C, 4), (C, 3) and (C, 2) give
 #define LN_MOST4(TX, TY)                                                                            \
   LN_CASE(TX, TY, 16, 1) LN_CASE(TX, TY, 16, 2) LN_CASE(TX, TY, 16, 3) LN_CASE(TX, TY, 16, 4)       \
-  LN_CASE(TX, TY, 32, 3) LN_CASE(TX, TY, 32, 4) LN_CASE(TX, TY, 64, 3) LN_CASE(TX, TY, 64, 4) LN_WIDE(TX, TY)
+  LN_CASE(TX, TY, 32, 3) LN_CASE(TX, TY, 32, 4) LN_CASE(TX, TY, 64, 3) LN_CASE(TX, TY, 64, 4) LN_CASE(TX, TY, 128, 3)             \
+  LN_CASE(TX, TY, 128, 4) LN_CASE(TX, TY, 256, 3) LN_CASE(TX, TY, 256, 4)
 #define LN_MOST3(TX, TY)                                                                            \
   LN_CASE(TX, TY, 16, 1) LN_CASE(TX, TY, 16, 2) LN_CASE(TX, TY, 16, 3) LN_CASE(TX, TY, 32, 2)       \
-  LN_CASE(TX, TY, 32, 3) LN_CASE(TX, TY, 64, 2) LN_CASE(TX, TY, 64, 3) LN_CASE(TX, TY, 256, 1) LN_WIDE(TX, TY)
+  LN_CASE(TX, TY, 32, 3) LN_CASE(TX, TY, 64, 2) LN_CASE(TX, TY, 64, 3) LN_CASE(TX, TY, 128, 3) LN_CASE(TX, TY, 256, 1)             \
+  LN_CASE(TX, TY, 256, 2) LN_CASE(TX, TY, 256, 3) LN_CASE(TX, TY, 256, 4)
 #define LN_MOST2(TX, TY)                                                                            \
   LN_CASE(TX, TY, 16, 1) LN_CASE(TX, TY, 16, 2) LN_CASE(TX, TY, 32, 2) LN_CASE(TX, TY, 64, 2)       \
-  LN_CASE(TX, TY, 256, 1) LN_WIDE(TX, TY)
+  LN_CASE(TX, TY, 128, 2) LN_CASE(TX, TY, 256, 2) LN_CASE(TX, TY, 256, 3) LN_CASE(TX, TY, 256, 4)
 
 extern "C" int ovis_layernorm_train_forward(const void* x, long long ldx, const void* residual, long long ldr, const float* gamma,
                                             const float* beta, void* sum, void* y, float* stats, uint8_t* codes, uint8_t* scales,
@@ -402,7 +418,7 @@ extern "C" int ovis_layernorm_train_forward(const void* x, long long ldx, const 
 
 extern "C" long long ovis_layernorm_train_backward_workspace_bytes(long long rows, int C, int x_dtype) {
   if (rows <= 0 || C <= 0 || C > 8192 || !ovis::dtype_ok(x_dtype)) return 0;
-  return (long long)bwd_blocks(rows, bwd_row_shape(C, x_dtype)) * 2 * C * 4;
+  return (long long)bwd_blocks(rows, bwd_row_shape(C, x_dtype), x_dtype) * 2 * C * 4;
 }
 
 extern "C" int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x, long long ldx, const uint8_t* codes,
@@ -416,7 +432,7 @@ extern "C" int ovis_layernorm_train_backward(const void* dy, long long lddy, con
   OVIS_REQUIRE(ovis::dtype_ok(dy_dtype) && ovis::dtype_ok(x_dtype) && (x_dtype == OVIS_F32 || x_dtype == dy_dtype),
                "layernorm_train_backward: dy has x's type, or any where x is f32");
   const RowShape sh = bwd_row_shape(C, x_dtype);
-  const unsigned blocks = bwd_blocks(rows, sh);
+  const unsigned blocks = bwd_blocks(rows, sh, x_dtype);
   float* to = blocks == 1 && dbeta == dgamma + C ? dgamma : workspace;
 #define LN_GO(TX, TY, LPR, NCH)                                                                                                             \
   if (codes && C % 8) LN_RUN(TX, TY, true, true, LPR, NCH);                                                                                 \
@@ -424,7 +440,7 @@ extern "C" int ovis_layernorm_train_backward(const void* dy, long long lddy, con
   else if (C % 8) LN_RUN(TX, TY, false, true, LPR, NCH);                                                                                    \
   else LN_RUN(TX, TY, false, false, LPR, NCH)
 #define LN_RUN(TX, TY, CK, TAIL, LPR, NCH)                                                                                                  \
-  hipLaunchKernelGGL((layernorm_train_bwd_kernel<TX, TY, CK, TAIL, LPR, NCH, bwd_waves(NCH)>), dim3(blocks),                                \
+  hipLaunchKernelGGL((layernorm_train_bwd_kernel<TX, TY, CK, TAIL, LPR, NCH, bwd_waves(NCH, sizeof(TX) == 4)>), dim3(blocks),                                \
                      dim3(256), 2 * LPR * NCH * 8 * 4, (hipStream_t)stream, (const TY*)dy, lddy, (const TX*)x, ldx, codes, scales, stats,   \
                      gamma, (const TX*)dsum, ldds, (TX*)dx, to, rows, C)
   LN_TYPES(x_dtype, dy_dtype, LN_MOST2, LN_MOST3)

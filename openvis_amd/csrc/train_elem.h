@@ -194,6 +194,8 @@ __device__ __forceinline__ void store_codes(uint8_t* __restrict__ p, int n, u32x
 }
 
 // sums the P lines of part [P][W] in a fixed order: columns below `split` to out0, the others to out1 (layernorm_train.hip)
+struct ColumnSum { const float* part; int P, W; float* out0; int split; float* out1; };
+int column_sum_two(const ColumnSum& a, const ColumnSum& b, hipStream_t stream);         // two of them in one launch
 int column_sum_finish(const float* part, int P, int W, float* out0, int split, float* out1, hipStream_t stream);
 
 // a launch's lanes along a dimension are counted in 32 bits: so many workgroups of 256 lanes at most

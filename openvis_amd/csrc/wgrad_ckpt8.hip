@@ -414,10 +414,26 @@ scale_tops_kernel(const uint8_t* __restrict__ scales, uint8_t* __restrict__ tops
   tops[i] = (uint8_t)t;
 }
 
-// dw = gamma sum over the parts + beta db
+// dw = gamma sum over the parts + beta db.  Workgroups from `joins` on: db = the sum of the lines of dbp, where dw does not need it
 __global__ void __launch_bounds__(256)
 wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict__ db, const float* __restrict__ gamma, const float* __restrict__ beta,
-                  float* __restrict__ dw, long long NK, int K) {
+                  float* __restrict__ dw, long long NK, int K, unsigned joins, const float* __restrict__ dbp, int lines, int N, float* __restrict__ dbo) {
+  if (blockIdx.x >= joins) {                                     // 16 columns, 16 lanes each
+    __shared__ float buf[16][17];
+    const int c = threadIdx.x & 15, l = threadIdx.x >> 4, w = (int)(blockIdx.x - joins) * 16 + c;
+    float s = 0.f;
+    if (w < N)
+#pragma unroll 8
+      for (int p = l; p < lines; p += 16) s += dbp[(long long)p * N + w];
+    buf[l][c] = s;
+    __syncthreads();
+    if (l == 0 && w < N) {
+#pragma unroll
+      for (int i = 1; i < 16; ++i) s += buf[i][c];
+      dbo[w] = s;
+    }
+    return;
+  }
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= NK) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -510,7 +526,7 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
                K, lddy, dtype);
   const WgradShape w = wgrad_shape(M, N, K, dtype);
   const long long blocks = (long long)w.tiles_n * w.tiles_k * w.S;
-  OVIS_REQUIRE(blocks <= ovis::kMostBlocks && (long long)N * K < (1ll << 34) && lddy < (1ll << 24) && K < (1 << 24), "linear_wgrad_ckpt8: %d x %d (row stride %lld) is too large for one call", N,
+  OVIS_REQUIRE(blocks <= ovis::kMostBlocks && (long long)N * K < (1ll << 33) && lddy < (1ll << 24) && K < (1 << 24), "linear_wgrad_ckpt8: %d x %d (row stride %lld) is too large for one call", N,
                K, lddy);
   const bool join = w.S > 1 || gamma;
   float* part = join ? workspace : dw;
@@ -552,17 +568,21 @@ extern "C" int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uin
   }
 #undef WG_GO
   int rc = ovis::check_launch("linear_wgrad_ckpt8");
-  if (rc == OVIS_OK && lines > 1) rc = ovis::column_sum_finish(dbp, lines, N, db, N, db, (hipStream_t)stream);
-  if (rc != OVIS_OK || !join) return rc;
+  if (rc != OVIS_OK) return rc;
   const long long NK = (long long)N * K;
   int S = w.S;
-  if (S > 8 && NK < 65536) {                                     // few columns, many parts: 64 lanes a column (9000 x 64 x 64 in 141 parts: 57 us by one)
+  const bool tree = S > 8 && NK < 65536, later = join && !tree && !gamma;         // db's lines are added up beside dw's parts where that can be
+  if (lines > 1 && !tree && !later) rc = ovis::column_sum_finish(dbp, lines, N, db, N, db, (hipStream_t)stream);
+  if (rc != OVIS_OK || !join) return rc;
+  if (tree) {                                     // few columns, many parts: 64 lanes a column (9000 x 64 x 64 in 141 parts: 57 us by one)
     float* to = gamma ? workspace + sp.parts + sp.lines : dw;
-    rc = ovis::column_sum_finish(part, S, (int)NK, to, (int)NK, to, (hipStream_t)stream);
+    rc = ovis::column_sum_two({part, S, (int)NK, to, (int)NK, to}, {dbp, lines, N, db, N, db}, (hipStream_t)stream);
     if (rc != OVIS_OK || !gamma) return rc;
     part = to;
     S = 1;
   }
-  hipLaunchKernelGGL(wgrad_join_kernel, dim3(ovis::cdiv((NK + 3) / 4, 256)), dim3(256), 0, (hipStream_t)stream, part, S, db, gamma, beta, dw, NK, K);
+  const unsigned joins = ovis::cdiv((NK + 3) / 4, 256);
+  hipLaunchKernelGGL(wgrad_join_kernel, dim3(joins + (later && lines > 1 ? ovis::cdiv(N, 16) : 0)), dim3(256), 0, (hipStream_t)stream, part, S,
+                     gamma ? db : nullptr, gamma, beta, dw, NK, K, joins, dbp, lines, N, db);
   return ovis::check_launch("linear_wgrad_ckpt8");
 }

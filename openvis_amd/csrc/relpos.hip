@@ -178,14 +178,16 @@ relpos_bwd_kernel(const T* __restrict__ g, long long bs, long long hs, long long
 }
 
 // Windows: sum over a run of the batch, element by element (grid: pieces of the [H, N, N] plane, batch chunks), then over the pairs of each
-// bucket.
+// bucket.  The four wavefronts of a workgroup take the same 64 vectors and a quarter of the run each, so that a line of sums is written and read
+// again for four times as much of the batch.
 template <typename T>
 __global__ void __launch_bounds__(256)
 window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long long ld, float* __restrict__ part, int H, int N, int nvec,
                        long long B, long long chunk) {
   const long long span = (B - 1) * bs + (long long)(H - 1) * hs + (long long)(N - 1) * ld + N;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)H * N * nvec) return;
+  __shared__ float buf[3][64][9];
+  const int lane = threadIdx.x & 63, grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long all = (long long)H * N * nvec, at = (long long)blockIdx.x * 64 + lane, i = at < all ? at : all - 1;
   const int v = (int)(i % nvec);
   const long long hr = i / nvec;
   const int row = (int)(hr % N), h = (int)(hr / N), n = N - v * 8;
@@ -200,34 +202,45 @@ window_bias_sum_kernel(const T* __restrict__ g, long long bs, long long hs, long
   if (n < 8) {
     while (bv > b0 && here + (bv - 1) * bs + 8 > span) --bv;     // a step or two, or all where the batch is one entry broadcast
   }
-  long long b = b0;
+  long long b = b0 + grp;
 #pragma unroll 4
-  for (; b < bv; ++b) {
+  for (; b < bv; b += 4) {
     Raw8<T> x;
     x.load_all(p + b * bs, true);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] += x.at(e);
   }
-  for (; b < b1; ++b) {
+  for (; b < b1; b += 4) {
     float x[8];
     load8(p + b * bs, n, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] += x[e];
   }
+  if (grp)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) buf[grp - 1][lane][e] = acc[e];
+  __syncthreads();
+  if (grp || at >= all) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += buf[w][lane][e];
   store8(part + (((long long)blockIdx.y * H + h) * N + row) * N + v * 8, n, acc);
 }
 
-// A workgroup takes the pairs of one vertical offset and head: a lane the pairs (xi, xj), whose rows of ws elements it adds over the token rows
+// The sums come in `lines` parts (few: with more a launch adds them up first).  A workgroup takes the pairs of one vertical offset and head: a lane the pairs (xi, xj), whose rows of ws elements it adds over the token rows
 // yj, then one of the 2 ws - 1 horizontal offsets each.
 __global__ void __launch_bounds__(256)
-window_bias_finish_kernel(const float* __restrict__ sum, float* __restrict__ dtable, int H, int ws) {
+window_bias_finish_kernel(const float* __restrict__ sum, int lines, float* __restrict__ dtable, int H, int ws) {
   extern __shared__ float pair[];                                // [xi][xj]
   const int h = blockIdx.y, N = ws * ws, w = 2 * ws - 1, dy = (int)blockIdx.x - (ws - 1);          // yi - yj
   const int y0 = max(0, -dy), y1 = min(ws, ws - dy);             // yj
   for (int t = threadIdx.x; t < N; t += 256) {
     const int xi = t / ws, xj = t - xi * ws;
     float s = 0.f;
-    for (int yj = y0; yj < y1; ++yj) s += sum[((long long)h * N + (yj + dy) * ws + xi) * N + yj * ws + xj];
+    for (int l = 0; l < lines; ++l)
+#pragma unroll 4
+      for (int yj = y0; yj < y1; ++yj) s += sum[(((long long)l * H + h) * N + (yj + dy) * ws + xi) * N + yj * ws + xj];
     pair[t] = s;
   }
   __syncthreads();
@@ -263,9 +276,9 @@ inline SeqShape seq_shape(long long B, int H, int Nq, int Nk) {
 }
 struct WinShape { long long chunk; int chunks; };
 inline WinShape win_shape(long long B, int H, int N) {
-  const long long blocks = ((long long)H * N * ((N + 7) / 8) + 255) / 256;
+  const long long blocks = ((long long)H * N * ((N + 7) / 8) + 63) / 64;
   long long want = (2048 + blocks - 1) / blocks;
-  const long long most = (B + 3) / 4;
+  const long long most = (B + 15) / 16;
   if (want > most) want = most;
   if (want > 65535) want = 65535;
   WinShape s;
@@ -364,15 +377,16 @@ extern "C" int ovis_swin_relpos_bias_backward(const void* dbias, long long bs, l
   const long long W = (long long)H * N * N;
   OVIS_REQUIRE(W < (1ll << 31), "swin_relpos_bias_backward: %d heads of windows of %d are too large for one call", H, ws);
 #define RP_GO(T)                                                                                                                            \
-  hipLaunchKernelGGL((window_bias_sum_kernel<T>), dim3(ovis::cdiv((long long)H * N * nvec, 256), s.chunks), dim3(256), 0,                   \
+  hipLaunchKernelGGL((window_bias_sum_kernel<T>), dim3(ovis::cdiv((long long)H * N * nvec, 64), s.chunks), dim3(256), 0,                   \
                      (hipStream_t)stream, (const T*)dbias, bs, hs, ld, workspace + W, H, N, nvec, B, s.chunk);
   RP_TYPE(dtype, RP_GO)
 #undef RP_GO
   int rc = ovis::check_launch("swin_relpos_bias_backward");
-  if (rc == OVIS_OK && s.chunks > 1)
+  const bool few = s.chunks <= 4;
+  if (rc == OVIS_OK && !few)
     rc = ovis::column_sum_finish(workspace + W, s.chunks, (int)W, workspace, (int)W, workspace, (hipStream_t)stream);
   if (rc != OVIS_OK) return rc;
   hipLaunchKernelGGL(window_bias_finish_kernel, dim3(2 * ws - 1, H), dim3(256), N * 4, (hipStream_t)stream,
-                     s.chunks > 1 ? workspace : workspace + W, dtable, H, ws);
+                     few ? workspace + W : workspace, few ? s.chunks : 1, dtable, H, ws);
   return ovis::check_launch("swin_relpos_bias_backward");
 }

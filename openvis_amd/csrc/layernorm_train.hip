@@ -8,7 +8,7 @@
 //   dgamma = sum over rows dy * xhat,  dbeta = sum over rows dy
 //
 // Bound by HBM: every input is read once and every output written once.  LPR neighbouring lanes hold a row in registers, 8 columns a lane and
-// NCH such pieces each (256 lanes = a whole workgroup from 2049 columns on), so a row is read once although forward needs it three times.
+// NCH such pieces each (up to 256 lanes, a whole workgroup), so a row is read once although forward needs it three times.
 // The weight gradient is summed over rows in a fixed order: a workgroup keeps the sums of its rows in registers, writes one line of the
 // workspace, and a second kernel adds the lines (no atomics: the same bits at every call).
 #include "train_elem.h"
@@ -136,7 +136,7 @@ layernorm_train_fwd_kernel(const TX* __restrict__ x, long long ldx, const TX* __
 // own: a mask in the other costs it the fetch ahead, 109 -> 144 us).  A workgroup walks over rows and keeps dgamma / dbeta of its lanes' columns
 // in registers, gamma in LDS.  The next row is fetched before the present one's sums begin, and rows stay in their stored width until they are
 // used: the sums take two dependent passes over a row, in which a wavefront without the next row's loads would have nothing in flight.
-// 98500 x 768 fp16 from 8 bits with dsum: 109 us, 4.9 TB/s (without the fetch ahead 133 us; a large copy reaches 5.0 TB/s).
+// 98500 x 768 fp16 from 8 bits with dsum: 108 us, 4.9 TB/s (without the fetch ahead 133 us; a large copy reaches 5.0 TB/s).
 template <typename TX, typename TY, bool CK, bool TAIL, int LPR, int NCH, int WAVES>
 __global__ void __launch_bounds__(256, WAVES)
 layernorm_train_bwd_kernel(const TY* __restrict__ dy, long long lddy, const TX* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
@@ -283,8 +283,9 @@ inline RowShape row_shape(int C, int most) {
   return {256, (nvec + 255) / 256};                              // C <= 8192: at most four
 }
 // Backward: a piece is 16 sums and two rows' dy, x and dsum: three pieces of 16-bit rows (220 registers) or two of f32 rows (192), two
-// wavefronts a SIMD; two pieces of 16-bit rows (165), three wavefronts (27286 x 4096: 147 us, with two wavefronts 169 us).  98500 x 768 fp16 in three pieces 133 us, in two 144 us; 73600 x 384 f32 in three 87 us, in two 83 us (before the fetch
-// ahead).  Rows of more than 4096 f32 or 6144 16-bit columns need more and spill.
+// wavefronts a SIMD; two pieces of 16-bit rows (165), three wavefronts (27286 x 4096: 147 us, with two wavefronts 169 us).  Before the fetch ahead
+// 98500 x 768 fp16 took 133 us in three pieces, 144 us in two; 73600 x 384 f32 87 us in three, 83 us in two.  Rows of more than 4096 f32 or 6144
+// 16-bit columns need more registers and spill.
 inline RowShape bwd_row_shape(int C, int x_dtype) { return row_shape(C, x_dtype == OVIS_F32 ? 2 : 3); }
 
 // as many workgroups as the card holds at once: each walks over its rows, and a workgroup that had to wait would walk alone at the end

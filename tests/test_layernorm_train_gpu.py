@@ -57,7 +57,7 @@ def _value8(ck):
 
 
 SHAPES = [(1, 1), (3, 2), (1, 7), (5, 31), (9, 33), (100, 256), (64, 128), (33, 191), (7, 192), (17, 384), (130, 512), (300, 768), (3, 1000),
-          (2051, 257), (5, 1536), (31, 2047), (6, 2049), (12, 4096), (3, 5001), (2, 8192)]
+          (2051, 257), (5, 1536), (31, 2047), (6, 2049), (12, 4096), (3, 5001), (2, 8192), (701, 2600), (300, 2051), (1501, 1111), (37, 3500), (900, 6150)]
 
 
 @pytest.mark.parametrize("rows,C", SHAPES)
@@ -89,7 +89,7 @@ def test_forward_and_backward(rows, C, xt, yt):
         _sum_close(db, rb, dy.double().abs().sum(0), rows, "dbeta")
 
 
-@pytest.mark.parametrize("rows,C", [(1, 1), (3, 31), (5, 33), (100, 256), (50, 257), (40, 768), (3, 2500), (2, 8191)])
+@pytest.mark.parametrize("rows,C", [(1, 1), (3, 31), (5, 33), (100, 256), (50, 257), (40, 768), (3, 2500), (2, 8191), (701, 2600), (300, 2051), (301, 1100), (40, 3501)])
 @pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")])
 def test_checkpoint_in_8_bits(rows, C, xt, yt):
     from openvis_amd import ops

@@ -153,19 +153,43 @@ at::Tensor msda_encoder_fused_meta(const at::Tensor& value, const at::Tensor&, c
 }
 
 // ---- attention_f16 -------------------------------------------------------------------------------------------------
-// q / k / v are VIEWS into fp16 buffers: element (b, row, h, d) sits at data_ptr + (b*bs + row*ld + h*D + d) halfs
+// q / k / v are VIEWS into fp16 buffers: element (b, row, h, d) sits at data_ptr + (b*bs + row*ld + h*D + d) halfs.
+// Strides that leave a tensor's storage are refused before the launch.  One case has a meaning of its own: the rows of such a view that were
+// copied (to(), clone(): a copy of a column slice is dense) and still come with the strides of the buffer they were cut from.  A tensor
+// [B N, >= H D] holds the same rows by its own stride, and is read by that.
+struct AttnRows { int64_t bs, ld; };
+AttnRows attn_rows(const char* what, const at::Tensor& t, int64_t B, int64_t N, int64_t H, int64_t D, int64_t bs, int64_t ld) {
+  TORCH_CHECK(bs >= 0 && ld >= 0, "attention_f16: negative stride of ", what);
+  const int64_t left = (int64_t)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
+  auto inside = [&](int64_t b, int64_t l) {
+    return (__int128)(B - 1) * b + (__int128)(N - 1) * l + (__int128)H * D <= (__int128)left;
+  };
+  if (inside(bs, ld)) return {bs, ld};
+  if (t.dim() == 2 && t.size(0) == B * N && t.size(1) >= H * D && t.stride(1) == 1 && inside(N * t.stride(0), t.stride(0))) return {N * t.stride(0), t.stride(0)};
+  TORCH_CHECK(false, "attention_f16: ", what, " ", t.sizes(), " does not hold ", B, " x ", N, " rows of ", H * D, " at the strides ", bs, " and ", ld);
+}
+struct AttnArgs { AttnRows q, k, v; };
+AttnArgs attn_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t D, int64_t q_bs,
+                   int64_t q_ld, int64_t k_bs, int64_t k_ld, int64_t v_bs, int64_t v_ld) {
+  for (const at::Tensor* t : {&q, &k, &v})
+    TORCH_CHECK(t->scalar_type() == at::kHalf && t->device() == q.device(), "attention_f16 needs fp16 tensors on one HIP device");
+  for (int64_t n : {B, H, Nq, Nk, D}) TORCH_CHECK(n > 0 && n < (1ll << 31), "attention_f16: a size of ", n);
+  for (int64_t l : {q_ld, k_ld, v_ld}) TORCH_CHECK(l < (1ll << 31), "attention_f16: a row stride of ", l);
+  return {attn_rows("q", q, B, Nq, H, D, q_bs, q_ld), attn_rows("k", k, B, Nk, H, D, k_bs, k_ld), attn_rows("v", v, B, Nk, H, D, v_bs, v_ld)};
+}
 at::Tensor attention_f16(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t D,
                          int64_t q_bs, int64_t q_ld, int64_t k_bs, int64_t k_ld, int64_t v_bs, int64_t v_ld) {
-  for (const at::Tensor* t : {&q, &k, &v}) TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kHalf, "attention_f16 needs fp16 HIP tensors");
+  const AttnArgs a = attn_args(q, k, v, B, H, Nq, Nk, D, q_bs, q_ld, k_bs, k_ld, v_bs, v_ld);
   c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   at::Tensor out = at::empty({B, Nq, H * D}, q.options());
-  const int rc = ovis_attention_f16(q.data_ptr(), q_bs, (int)q_ld, k.data_ptr(), k_bs, (int)k_ld, v.data_ptr(), v_bs, (int)v_ld, out.data_ptr(),
+  const int rc = ovis_attention_f16(q.data_ptr(), a.q.bs, (int)a.q.ld, k.data_ptr(), a.k.bs, (int)a.k.ld, v.data_ptr(), a.v.bs, (int)a.v.ld, out.data_ptr(),
                                     Nq * H * D, (int)(H * D), (int)B, (int)H, (int)Nq, (int)Nk, (int)D, 1.0f / std::sqrt((float)D), cur_stream());
   TORCH_CHECK(rc == OVIS_OK, "attention_f16: ", ovis_last_error());
   return out;
 }
-at::Tensor attention_f16_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor&, int64_t B, int64_t H, int64_t Nq, int64_t, int64_t D,
-                              int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) {
+at::Tensor attention_f16_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t B, int64_t H, int64_t Nq, int64_t Nk, int64_t D,
+                              int64_t q_bs, int64_t q_ld, int64_t k_bs, int64_t k_ld, int64_t v_bs, int64_t v_ld) {
+  attn_args(q, k, v, B, H, Nq, Nk, D, q_bs, q_ld, k_bs, k_ld, v_bs, v_ld);
   return at::empty({B, Nq, H * D}, q.options());
 }
 

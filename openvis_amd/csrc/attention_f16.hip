@@ -144,7 +144,7 @@ flash_attn_f16_kernel(AttnH a) {
       ps += p;
     }
     ps += __shfl_xor(ps, 32, 64);
-    l_run = l_run * alpha + ps;
+    l_run = __builtin_fmaf(l_run, alpha, ps);
     m_run = m_new;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -310,7 +310,7 @@ flash_attn_f16_seq_kernel(AttnH a) {
         }
       }
     ps = sum_xor32(ps);
-    l_run = l_run * alpha + ps;
+    l_run = __builtin_fmaf(l_run, alpha, ps);
     m_run = m_new;
 #pragma unroll
     for (int t = 0; t < 2; ++t)

@@ -32,6 +32,22 @@ __device__ __forceinline__ unsigned xcd_remap(unsigned bid, unsigned nblk) {
   return base + (bid >> 3);
 }
 
+// a * b rounded by itself: the compiler does not fuse it with an addition.  Where a sum of products feeds outputs that are compared bit by bit,
+// which product is fused with which addition is written out with this and fmaf instead of left to the compiler, whose choice changes
+// with its flags (and, by the vector width it tries first, from one component of a float4 to the next).
+__device__ __forceinline__ float mul_rn(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// the four taps of a bilinear interpolation, hy (hx a + lx b) + ly (hx c + lx d), in the two orders of rounding that are in use
+__device__ __forceinline__ float bilinear_top(float hy, float ly, float hx, float lx, float a, float b, float c, float d) {
+  return __builtin_fmaf(ly, __builtin_fmaf(hx, c, mul_rn(lx, d)), mul_rn(hy, __builtin_fmaf(lx, b, mul_rn(hx, a))));
+}
+__device__ __forceinline__ float bilinear_bottom(float hy, float ly, float hx, float lx, float a, float b, float c, float d) {
+  return __builtin_fmaf(hy, __builtin_fmaf(hx, a, mul_rn(lx, b)), mul_rn(ly, __builtin_fmaf(hx, c, mul_rn(lx, d))));
+}
+
 inline unsigned cdiv(long long a, long long b) { return (unsigned)((a + b - 1) / b); }
 
 // "fp16x2" arithmetic of a large f32 GEMM (gemm_f16_pp.hip FH, gemm_f32x3.h FH): activations are multiplied by a_scale while they are split

@@ -711,7 +711,7 @@ gemm_f16_pp_kernel(const PPArgs p) {
         asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:16\n\ts_waitcnt lgkmcnt(0)" : "=&v"(t0), "=&v"(t1) : "v"(rbase + (unsigned)mb * 512u) : "memory");
         const float S1 = (t0[0] + t0[2]) + (t1[0] + t1[2]), S2 = (t0[1] + t0[3]) + (t1[1] + t1[3]);
         const float mean = S1 * (1.f / 256.f);
-        const float var = fmaxf(S2 * (1.f / 256.f) - mean * mean, 0.f);
+        const float var = fmaxf(__builtin_fmaf(-mean, mean, S2 * (1.f / 256.f)), 0.f);      // mean^2 is not rounded
         const float rstd = 1.f / sqrtf(var + p.lno_eps);
         // gamma / beta of the lane's 16 columns, re-read per row block (eight LDS reads in flight, one wait): held across the whole
         // epilogue they cost 32 registers on top of the accumulators and spill

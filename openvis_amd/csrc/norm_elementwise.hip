@@ -105,7 +105,9 @@ layernorm_kernel(const float* __restrict__ x, const float* __restrict__ res, con
     const int idx = lane + i * 64;
     if (idx < nv) {
       const float a = v[i].x - mean, b = v[i].y - mean, c = v[i].z - mean, d = v[i].w - mean;
-      q += (a * a + b * b) + (c * c + d * d);
+      // the squares' roundings are written out (f32 rows of one vector a lane: each by itself): what follows is compared bit by bit
+      if constexpr (MAXV == 1 && !OUT16) q += (ovis::mul_rn(a, a) + ovis::mul_rn(b, b)) + (ovis::mul_rn(c, c) + ovis::mul_rn(d, d));
+      else q += __builtin_fmaf(a, a, ovis::mul_rn(b, b)) + __builtin_fmaf(c, c, ovis::mul_rn(d, d));
     }
   }
   const float rstd = 1.f / sqrtf(wave_sum(q) / (float)C + eps);
@@ -167,7 +169,7 @@ layernorm_h16_kernel(const _Float16* __restrict__ x, const float* __restrict__ g
   for (int i = 0; i < NV8; ++i) {
     if (lane + i * 64 < n8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q += d * d; }
+      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q += ovis::mul_rn(d, d); }      // the squares rounded: compared bit by bit
     }
   }
   const float rstd = 1.f / sqrtf(wave_sum(q) / (float)C + eps);
@@ -219,7 +221,7 @@ row_stats_h16_kernel(const _Float16* __restrict__ x, float2* __restrict__ stats,
   for (int i = 0; i < NV8; ++i) {
     if (lane + i * 64 < n8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q += d * d; }
+      for (int e = 0; e < 8; ++e) { const float d = v[i][e] - mean; q += ovis::mul_rn(d, d); }      // the squares rounded: compared bit by bit
     }
   }
   const float rstd = 1.f / sqrtf(wave_sum(q) / (float)C + eps);
@@ -331,10 +333,11 @@ gn_apply_kernel(const float* __restrict__ x, const double* __restrict__ stats, c
     const float4* ub = reinterpret_cast<const float4*>(up + (long long)n * UH * UW * C);
     const float4 a = ub[((long long)y0 * UW + x0) * c4n + cq], b = ub[((long long)y0 * UW + x1) * c4n + cq];
     const float4 c = ub[((long long)y1 * UW + x0) * c4n + cq], d = ub[((long long)y1 * UW + x1) * c4n + cq];
-    o.x += hy * (hx * a.x + lx * b.x) + ly * (hx * c.x + lx * d.x);
-    o.y += hy * (hx * a.y + lx * b.y) + ly * (hx * c.y + lx * d.y);
-    o.z += hy * (hx * a.z + lx * b.z) + ly * (hx * c.z + lx * d.z);
-    o.w += hy * (hx * a.w + lx * b.w) + ly * (hx * c.w + lx * d.w);
+    // the sums' roundings are written out: output masks are compared bit by bit, and single pixels follow them
+    o.x += ovis::bilinear_top(hy, ly, hx, lx, a.x, b.x, c.x, d.x);
+    o.y += ovis::bilinear_bottom(hy, ly, hx, lx, a.y, b.y, c.y, d.y);
+    o.z += ovis::bilinear_top(hy, ly, hx, lx, a.z, b.z, c.z, d.z);
+    o.w += ovis::bilinear_bottom(hy, ly, hx, lx, a.w, b.w, c.w, d.w);
   }
   if (relu) { o.x = fmaxf(o.x, 0.f); o.y = fmaxf(o.y, 0.f); o.z = fmaxf(o.z, 0.f); o.w = fmaxf(o.w, 0.f); }
   reinterpret_cast<float4*>(y)[oidx] = o;

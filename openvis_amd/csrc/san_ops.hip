@@ -117,10 +117,11 @@ resize_add_kernel(float* __restrict__ dst, const float* __restrict__ src, int N,
   const float4 a = sb[((long long)y0 * w + x0) * c4n + cq], b = sb[((long long)y0 * w + x1) * c4n + cq];
   const float4 c = sb[((long long)y1 * w + x0) * c4n + cq], d = sb[((long long)y1 * w + x1) * c4n + cq];
   float4 v = reinterpret_cast<float4*>(dst)[i];
-  v.x += hy * (hx * a.x + lx * b.x) + ly * (hx * c.x + lx * d.x);
-  v.y += hy * (hx * a.y + lx * b.y) + ly * (hx * c.y + lx * d.y);
-  v.z += hy * (hx * a.z + lx * b.z) + ly * (hx * c.z + lx * d.z);
-  v.w += hy * (hx * a.w + lx * b.w) + ly * (hx * c.w + lx * d.w);
+  // the sums' roundings are written out: output masks are compared bit by bit, and single pixels follow them
+  v.x += ovis::bilinear_top(hy, ly, hx, lx, a.x, b.x, c.x, d.x);
+  v.y += ovis::bilinear_bottom(hy, ly, hx, lx, a.y, b.y, c.y, d.y);
+  v.z += ovis::bilinear_top(hy, ly, hx, lx, a.z, b.z, c.z, d.z);
+  v.w += __builtin_fmaf(hy, __builtin_fmaf(lx, b.w, ovis::mul_rn(hx, a.w)), ovis::mul_rn(ly, __builtin_fmaf(hx, c.w, ovis::mul_rn(lx, d.w))));
   reinterpret_cast<float4*>(dst)[i] = v;
 }
 

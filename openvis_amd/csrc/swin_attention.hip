@@ -89,7 +89,7 @@ swin_window_attn_kernel(const _Float16* __restrict__ qkv, _Float16* __restrict__
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool dead = key0 + e >= N || ((mk >> (8 * e)) & 0xffu);
-        const float x = dead ? -INFINITY : s[4 * g + e] * sl2 + bb[e] * l2e;
+        const float x = dead ? -INFINITY : __builtin_fmaf(bb[e], l2e, ovis::mul_rn(s[4 * g + e], sl2));
         s[4 * g + e] = x;
         mt = fmaxf(mt, x);
       }
@@ -106,7 +106,7 @@ swin_window_attn_kernel(const _Float16* __restrict__ qkv, _Float16* __restrict__
       ps += p;
     }
     ps += __shfl_xor(ps, 32, 64);
-    sum = sum * alpha + ps;
+    sum = __builtin_fmaf(sum, alpha, ps);
     m_run = m_new;
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[r] *= alpha;

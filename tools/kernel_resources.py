@@ -5,7 +5,7 @@ import subprocess
 import sys
 
 src, flt = sys.argv[1], (sys.argv[2] if len(sys.argv) > 2 else "")
-r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-c", src, "-o", "/dev/null",
+r = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-c", src, "-o", "/dev/null",
                     "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True)
 PATS = {"VGPR": r" VGPRs: (\d+)", "AGPR": r"AGPRs: (\d+)", "spill": r"VGPR Spill: (\d+)", "scratch": r"ScratchSize \[bytes/lane\]: (\d+)",
         "LDS": r"LDS Size \[bytes/block\]: (\d+)", "occ": r"Occupancy \[waves/SIMD\]: (\d+)"}

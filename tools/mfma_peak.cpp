@@ -2,7 +2,7 @@
 // v_mfma_f32_16x16x32_f16 on register operands, 16 accumulators per wavefront, 1 or 2 wavefronts per SIMD, every CU busy.
 // The chip lowers its clock under MFMA load (MI355X_MICROARCH.md, DVFS give-back), so this -- not 2.5 PF -- is the ceiling a
 // GEMM kernel on real activations can approach; the same loop on zero operands shows the clock it would otherwise hold.
-//   hipcc --offload-arch=gfx950 -O2 tools/mfma_peak.cpp -o build/mfma_peak && ./build/mfma_peak
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/mfma_peak.cpp -o build/mfma_peak && ./build/mfma_peak
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

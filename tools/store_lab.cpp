@@ -1,5 +1,5 @@
 // store_lab: how fast can one CU issue the epilogue stores of a 256x256 GEMM tile, by store shape?
-//   hipcc --offload-arch=gfx950 -O2 tools/store_lab.cpp -o build/store_lab
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/store_lab.cpp -o build/store_lab
 // Every workgroup (512 threads, one per CU) "stores a tile" `iters` times; a wave owns 128 rows x ROWB bytes per tile
 // (ROWB = 128: fp16 outputs of 64 columns, 256: f32).  Patterns: rows covered by one 1-KB wave-instruction.
 #include <hip/hip_runtime.h>

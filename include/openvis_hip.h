@@ -581,7 +581,7 @@ int ovis_layernorm_train_backward(const void* dy, long long lddy, const void* x,
 /* An MLP's activation function with its input kept in 8 bits (act codes as above; the reference trains ReLU FFNs, msdeformattn.py:118-121,
  * QuickGELU, model.py:232-234, and GELU, swin.py:21-41).
  *   forward: y [rows, C] = act(h), codes / scales = h in 8 bits; act 0 with y NULL: the 8-bit form alone.  With ReLU the sign bit of a code
- *     says that the value was not positive.  h, y and dy, dh have one type.
+ *     says that the value was not positive, and -infinity is kept as -0 (its activation and its slope are 0).  h, y and dy, dh have one type.
  *   backward: dh = dy act'(value of the code), dbias f32 [C] = sum over rows of dh before its rounding (fixed order), codes_out / scales_out
  *     (both or neither NULL) = act(value of the code) in 8 bits; workspace of ovis_act_ckpt8_backward_workspace_bytes(rows, C) bytes.
  *   decode: out [rows, C] = the values that the codes stand for, rounded to dtype. */

@@ -5,7 +5,7 @@
 //             weight gradient, which then need not be kept either)
 //
 //   ReLU       act' = 1 where the code's sign bit is clear: the forward pass gives values that are not positive a set sign bit, so the
-//              derivative is that of h itself even where its code underflows to 0
+//              derivative is that of h itself even where its code underflows to 0 or h is -infinity (kept as -0; a NaN lets the gradient pass)
 //   QuickGELU  act = h g, act' = g (1 + 1.702 h (1 - g)),  g = 1 / (1 + exp(-1.702 h))
 //   GELU       act = h Phi, act' = Phi + h phi,  phi = exp(-h^2 / 2) / sqrt(2 pi), Phi = phi's integral
 //
@@ -41,7 +41,7 @@ template <int ACT>
 __device__ __forceinline__ void activation(float h, float& y, float& slope) {
   if constexpr (ACT == 1) {
     y = h < 0.f ? 0.f : h;                                       // passes a NaN on
-    slope = (__builtin_bit_cast(unsigned, h) >> 31) ? 0.f : 1.f;
+    slope = h == h && (__builtin_bit_cast(unsigned, h) >> 31) ? 0.f : 1.f;           // a decoded NaN has a sign of its own
   } else if constexpr (ACT == 2) {
     const float g = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.702f * kLog2e * h));
     y = h * g;

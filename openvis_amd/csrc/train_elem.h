@@ -7,7 +7,8 @@
 // 8-bit block format: e4m3 codes and one power-of-two scale (e8m0: 2^(byte - 127)) per 32 columns of a row.  Four neighbouring lanes hold a
 // block.  The scale is the smallest power of two in [2^-100, 2^120] under which the block's largest finite magnitude is at most 448, so no
 // value saturates and every value above 2^-6 of its scale is off by at most 2^-4 of itself.  The limits keep scale, value and their product
-// inside f32's normal range.  e4m3 has no infinity: infinities and NaN become the NaN code and do not take part in the block's maximum.
+// inside f32's normal range.  e4m3 has no infinity: infinities and NaN become the NaN code (-infinity in front of a ReLU: -0) and do not take part
+// in the block's maximum.
 // (Values from 2^128 (1 - 2^-5) on round to a code that stands for 2^128, an infinity in f32.)
 #pragma once
 #include "common.h"
@@ -107,7 +108,8 @@ __device__ __forceinline__ unsigned quad_max(unsigned a) {
 __device__ __forceinline__ unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
 
 // 8 values of one lane (the block's other 24 in its three neighbours; all four lanes active) -> 8 codes, and the scale's byte.
-// signed_zero: a value of 0 gets the code -0, so that a code's sign bit says "not positive" (ReLU's derivative).
+// signed_zero: a value of 0 gets the code -0, so that a code's sign bit says "not positive" (ReLU's derivative).  So does -infinity, whose ReLU
+// and whose derivative are 0 like those of any value below 0: as a NaN it would come back where the forward pass gave 0.
 // The maximum is taken over the magnitudes' bits: they order as the values do, with infinity and then every NaN (signalling ones too, which
 // a floating-point maximum would pass on) at the top.
 __device__ __forceinline__ u32x2_u encode8(const float (&v)[8], bool signed_zero, unsigned& scale_byte) {
@@ -119,13 +121,15 @@ __device__ __forceinline__ u32x2_u encode8(const float (&v)[8], bool signed_zero
   float w[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = v[e];
+  u32x2_u keep = {~0u, ~0u};
   if (a >= kInf) {                                                 // rare: the maximum of the finite ones, the others to NaN
     a = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool fine = magnitude(w[e]) < kInf;
       a = max(a, fine ? magnitude(w[e]) : 0u);
-      w[e] = fine ? w[e] : NAN;
+      w[e] = fine ? w[e] : signed_zero && v[e] < 0.f ? -0.f : NAN;
+      if (w[e] != w[e]) keep[e >> 2] &= ~(0x80u << (8 * (e & 3)));  // the conversion sets a NaN's sign, which is for "not positive" alone
     }
     a = quad_max(a);
   }
@@ -142,6 +146,7 @@ __device__ __forceinline__ u32x2_u encode8(const float (&v)[8], bool signed_zero
   t = __builtin_amdgcn_cvt_pk_fp8_f32(w[4], w[5], 0, false);
   t = __builtin_amdgcn_cvt_pk_fp8_f32(w[6], w[7], t, true);
   r[1] = (unsigned)t;
+  r[0] &= keep[0], r[1] &= keep[1];
   return r;
 }
 

@@ -1096,7 +1096,8 @@ def ckpt8_decode(ck, dtype=torch.float32):
 
 
 def act_forward_ckpt8(h, act):
-    """The activation of an MLP (ACT_RELU, ACT_QUICKGELU or ACT_GELU), for training: h [..., C] -> (y = act(h) in h's type, h as a Ckpt8)."""
+    """The activation of an MLP (ACT_RELU, ACT_QUICKGELU or ACT_GELU), for training: h [..., C] -> (y = act(h) in h's type, h as a Ckpt8).  With
+    ACT_RELU the sign bit of a code says that h was not positive, and -infinity is kept as -0."""
     if act == ACT_NONE:
         raise _lib.OvisError("act_forward_ckpt8: act must be ACT_RELU, ACT_QUICKGELU or ACT_GELU")
     y, codes, scales = _train("act_forward_ckpt8", h, act)

@@ -9,7 +9,10 @@
 // LDS read.  X is widened while it is staged, where 32 neighbouring columns share a scale: to bf16 (4 significant bits and any scale: exact).
 //   dY bf16: one bf16 product.  dY f32: three (f32 = the sum of three bf16 numbers), f32-grade.
 //   dY fp16: fp16 products; X is scaled per 32 columns by the largest scale of the workgroup's rows so that its largest code comes to at most
-//   57344: exact for scales down to 2^-22 of the largest, below that off by at most 2^-30 of the 32 columns' largest value.
+//   57344: exact for scales down to 2^-22 of the largest.  A workgroup that meets a smaller one (rows far apart in size, the large ones perhaps
+//   with no gradient at all) throws its sums away and takes its rows again with dY as the sum of two bf16 numbers (11 bits: exact), which
+//   takes five times as long.  Blocks of the format's smallest scale, 2^-100, do not count: they are the zeros of padding and of ReLU; what
+//   values they hold, below 2^-91, are taken as 0 where the 32 columns' largest scale is 2^-77 or more.
 // All products are exact in f32; sums are f32.  Rows are split over workgroups (S parts) where there are too few tiles to fill the card; the
 // parts are added in a fixed order by a second kernel.  36928 x 1024 x 4096 fp16: 270 us, 1.15 PFLOP/s (2000 x 1000 x 1000: 27 us).
 #include "train_elem.h"
@@ -176,6 +179,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
   const int yr = tid / (TN / 8), yc = (tid % (TN / 8)) * 8, xr = tid / (TK / XC), xc = (tid % (TK / XC)) * XC;
   const int yn = N - n0 - yc, xn = K - k0 - xc;                  // columns from this lane's first on
   const int xtop = F16 ? top[xc >> 5] - 7 : 0;
+  int lowest = 0;                                                // the smallest exponent that codes are widened with, blocks of the smallest scale aside
   struct Rows { DyOf<T> y[YP]; u32x2_u x[XP]; unsigned s; };
   // no masks; a step's uniform row pointers and a lane's 32-bit offsets from them; in pieces, to lie between the products
   struct At { const T* y; const uint8_t *c, *s; };
@@ -212,7 +216,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
       const int n = ok ? xn - 8 * j : 0;
       R.x[j] = load_codes(codes + (n > 0 ? r * K + k0 + xc + 8 * j : 0), n);
     }
-    R.s = ok ? scales[r * nblk + ((k0 + xc) >> 5)] : 27u;
+    R.s = ok ? scales[r * nblk + ((k0 + xc) >> 5)] : F16 ? (unsigned)xtop : 127u;
   };
   float dsum[8];
 #pragma unroll
@@ -235,6 +239,7 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
         *reinterpret_cast<u16x8*>(ly + (buf * P + p) * BM * TN + at<TN>(yr + i * YR, yc)) = R.y[i].plane(p);
     } else {
       const int j = i - YP, sb = (int)(R.s & 0xffu), e = F16 ? max(sb - xtop, -60) : sb - 127;      // 60 octaves below the largest nothing is left in fp16
+      if constexpr (F16) lowest = min(lowest, sb == 27 ? 0 : e);
       *reinterpret_cast<u16x8*>(lx + buf * BM * TK + at<TK>(xr, xc + 8 * j)) = widen<F16>(R.x[j], pow2f(e));
     }
   };
@@ -367,12 +372,57 @@ wgrad_ckpt8_kernel(const T* __restrict__ dy, long long lddy, const uint8_t* __re
     __syncthreads();
   }
 
+  // fp16's last bit is 2^-24 and a code's 2^-9: where all exponents were -15 or more, nothing was lost
+  bool wide = false;
+  if constexpr (F16) {
+    wide = __syncthreads_or(xn > 0 && lowest < -15) != 0;
+    if (wide) {                                                  // the chunk's rows again, in bf16: dY's two terms in the first two buffers
+#pragma unroll
+      for (int a = 0; a < AN; ++a)
+#pragma unroll
+        for (int b = 0; b < AK; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+      for (long long m = m0; m < m1; m += BM) {
+        Rows R;
+        fetch_masked(R, m);
+#pragma unroll
+        for (int i = 0; i < YP; ++i) {
+          u16x8 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = R.y[i].value(e), rest = v - (float)(__bf16)v;
+            hi[e] = __builtin_bit_cast(unsigned short, (__bf16)v);
+            lo[e] = __builtin_bit_cast(unsigned short, (__bf16)(rest == rest ? rest : 0.f));          // of an infinity or a NaN: none
+          }
+          *reinterpret_cast<u16x8*>(ly + at<TN>(yr + i * YR, yc)) = hi;
+          *reinterpret_cast<u16x8*>(ly + BM * TN + at<TN>(yr + i * YR, yc)) = lo;
+        }
+#pragma unroll
+        for (int j = 0; j < XP; ++j) *reinterpret_cast<u16x8*>(lx + at<TK>(xr, xc + 8 * j)) = widen<false>(R.x[j], pow2f((int)(R.s & 0xffu) - 127));
+        __syncthreads();
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+          Frags F;
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+#pragma unroll
+            for (int i = p ? AK : 0; i < NR; ++i) read_piece(F, p, st, i);
+#pragma unroll
+            for (int g = 0; g < G; ++g) acc[g / AK][g % AK] = mfma<false>(F.a[0][g / AK], F.b[g % AK], acc[g / AK][g % AK]);
+          }
+        }
+        __syncthreads();
+      }
+    }
+  }
+
   // a lane holds column k = lane & 31 of its blocks; register r is row (r & 3) + 8 (r >> 2) + 4 half
   float* o = out + s * N * K;
 #pragma unroll
   for (int b = 0; b < AK; ++b) {
     const int kl = wk * RK + b * 32, k = k0 + kl + (lane & 31);
-    const float f = F16 ? pow2f(top[kl >> 5] - 127 - 7) : 1.f;
+    const float f = F16 && !wide ? pow2f(top[kl >> 5] - 127 - 7) : 1.f;
     if (k < K) {
 #pragma unroll
       for (int a = 0; a < AN; ++a)

@@ -615,7 +615,8 @@ int ovis_swin_relpos_bias_backward(const void* dbias, long long bs, long long hs
 /* Weight gradient of a linear layer (y = x W^T + b, W [N, K]) from its input in 8 bits: dw f32 [N, K] = sum over rows dy[m, n] x[m, k],
  * db f32 [N] = sum dy; dy [M, N] (row stride lddy), codes / scales the 8-bit form of x [M, K].  gamma, beta f32 [K] (both or neither NULL):
  * the codes are a layer norm's normalised rows and the layer's input was x gamma + beta: dw = gamma sum dy x + beta db.  Products exact
- * at every scale (fp16 dy: but blocks of the smallest scale, 2^-100, count as 0 where another of these 32 columns' has 2^-77 or more),
+ * at every scale (fp16 dy: but blocks of the smallest scale, 2^-100, count as 0 where another of these 32 columns' has 2^-77 or more;
+ * f32 dy: values below 2^-110 are off by at most 2^-133, an infinity gives NaN),
  * f32 sums in a fixed order; workspace of ovis_linear_wgrad_ckpt8_workspace_bytes(M, N, K, dtype) bytes. */
 long long ovis_linear_wgrad_ckpt8_workspace_bytes(long long M, int N, int K, int dtype);
 int ovis_linear_wgrad_ckpt8(const void* dy, long long lddy, const uint8_t* codes, const uint8_t* scales, const float* gamma, const float* beta,

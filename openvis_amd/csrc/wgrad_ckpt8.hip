@@ -7,7 +7,8 @@
 // Bound by the matrix cores (2 M N K flop) when N and K are large.  Both operands lie with the summed dimension m along their rows, so a tile
 // of BM rows of each is laid row by row into LDS and the fragments, 8 consecutive m of one column a lane, come out through the transposing
 // LDS read.  X is widened while it is staged, where 32 neighbouring columns share a scale: to bf16 (4 significant bits and any scale: exact).
-//   dY bf16: one bf16 product.  dY f32: three (f32 = the sum of three bf16 numbers), f32-grade.
+//   dY bf16: one bf16 product.  dY f32: three (f32 = the sum of three bf16 numbers, exact for magnitudes from 2^-110 on; smaller ones are off by
+//   at most 2^-133, bf16's last bit; an infinity minus itself makes its column's sums NaN).
 //   dY fp16: fp16 products; X is scaled per 32 columns by the largest scale of the workgroup's rows so that its largest code comes to at most
 //   57344: exact for scales down to 2^-22 of the largest.  A workgroup that meets a smaller one (rows far apart in size, the large ones perhaps
 //   with no gradient at all) throws its sums away and takes its rows again with dY as the sum of two bf16 numbers (11 bits: exact), which
@@ -81,15 +82,16 @@ template <> struct DyOf<float> {
   }
   __device__ __forceinline__ void load_all(const float* p) { load8(p, 8, v); }
   __device__ __forceinline__ float value(int e) const { return v[e]; }
-  __device__ __forceinline__ u16x8 plane(int i) const {         // the i-th bf16 term of v (each the rest rounded to nearest)
+  // the i-th bf16 term of v, each the upper half of what is left: 8 of the 24 significant bits, so that the three are exact and none is larger than v
+  // (rounded to nearest the first term of values from 2^128 (1 - 2^-9) on would be an infinity)
+  __device__ __forceinline__ u16x8 plane(int i) const {
     u16x8 r;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float x = v[e];
-      __bf16 t = (__bf16)x;
-      if (i > 0) { x -= (float)t; t = (__bf16)x; }
-      if (i > 1) { x -= (float)t; t = (__bf16)x; }
-      r[e] = __builtin_bit_cast(unsigned short, t);
+#pragma unroll
+      for (int k = 0; k < i; ++k) x -= __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & 0xffff0000u);
+      r[e] = (unsigned short)(__builtin_bit_cast(unsigned, x) >> 16);
     }
     return r;
   }

@@ -45,7 +45,7 @@ __device__ __forceinline__ void activation(float h, float& y, float& slope) {
   } else if constexpr (ACT == 2) {
     const float g = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.702f * kLog2e * h));
     y = h * g;
-    slope = g * fmaf(1.702f * h, 1.f - g, 1.f);
+    slope = fmaf(1.702f, y * (1.f - g), g);                      // g (1 + 1.702 h (1 - g)), with no product above h
   } else if constexpr (ACT == 3) {
     float e, tail;
     gauss(h, e, tail);

@@ -37,3 +37,17 @@ def test_relu_of_infinities(dt, C):
     assert ((db.cpu().double() - want.double().sum(0)).abs() <= 6 * 2.0 ** -24 * want.double().abs().sum(0)).all()
     again = y8.codes.cpu().float()
     assert torch.equal(again[low], torch.zeros(int(low.sum()))) and torch.isfinite(again[~odd]).all() and torch.isnan(again[odd]).all()
+
+
+@pytest.mark.parametrize("act", ["quickgelu", "gelu"])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_the_largest_values(act, dt):
+    """values up to the 8-bit form's largest, 448 * 2^119: the activation is h or 0 and the slope 1 or 0, exactly, and none of it NaN"""
+    from openvis_amd import ops
+    code = {"quickgelu": ops.ACT_QUICKGELU, "gelu": ops.ACT_GELU}[act]
+    h = torch.tensor([[s * m * 2.0 ** e for m in (1.0, 1.25, 1.75) for s in (1, -1)] for e in (20, 63, 64, 100, 126, 127)])
+    y, ck = ops.act_forward_ckpt8(h.to(T[dt]).cuda(), code)
+    assert torch.equal(y.cpu().float(), h.clamp(min=0))
+    dh, db, y8 = ops.act_backward_ckpt8(torch.ones_like(y), ck, code, recompute=True)
+    assert torch.equal(dh.cpu().float(), (h > 0).float()) and torch.equal(db.cpu(), (h > 0).float().sum(0))
+    assert torch.equal(ops.ckpt8_decode(y8).cpu(), h.clamp(min=0))

@@ -7,6 +7,7 @@ import ctypes
 import functools
 import typing
 
+import numpy
 import torch
 
 from . import _lib
@@ -1121,7 +1122,7 @@ def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
 
 @functools.lru_cache(maxsize=64)
 def _relpos_borders(num_buckets, max_distance, bidirectional):
-    """int32 tensor on the host: the distances at which the buckets of a direction begin (bucket 0 is distance 0), counted in whole numbers: with
+    """int32 array: the distances at which the buckets of a direction begin (bucket 0 is distance 0), counted in whole numbers: with
     n = the direction's buckets and e = n // 2, bucket k < e is distance k; bucket e + k begins at the first d with
     (d / e)^(n - e) >= (max_distance / e)^k."""
     n = num_buckets // 2 if bidirectional else num_buckets
@@ -1140,7 +1141,22 @@ def _relpos_borders(num_buckets, max_distance, bidirectional):
             else:
                 lo = m + 1
         at.append(lo)
-    return torch.tensor(at, dtype=torch.int32)
+    return numpy.array(at, dtype=numpy.int32)
+
+
+_BORDERS = {}
+
+
+def _borders(*key):
+    """the borders as a host tensor, kept from call to call: made past the default device, and not kept where a mode in force makes it another kind"""
+    t = _BORDERS.get(key)
+    if t is None:
+        t = torch.from_numpy(_relpos_borders(*key))
+        if type(t) is torch.Tensor and t.device.type == "cpu":
+            if len(_BORDERS) >= 64:
+                _BORDERS.clear()
+            _BORDERS[key] = t
+    return t
 
 
 def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset=0, out_dtype=torch.float32, ld=None):
@@ -1150,7 +1166,7 @@ def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset
     logarithmically up to max_distance, the last bucket holds all that is farther.  bidirectional: the second half of the buckets is for keys
     behind the query (j > i + q_offset); otherwise those have distance 0.  q_offset: position of the first query among the keys (one new token of
     a cache: Nq = 1, q_offset = Nk - 1)."""
-    borders = _relpos_borders(table.shape[0] if table.dim() else 0, int(max_distance), bool(bidirectional))
+    borders = _borders(table.shape[0] if table.dim() else 0, int(max_distance), bool(bidirectional))
     if ld is not None and ld < max(Nk, 1):
         raise _lib.OvisError(f"relpos_bias_1d: ld must be at least {max(Nk, 1)}")
     return _train("relpos_bias_1d", table, borders, bool(bidirectional), Nq, Nk, q_offset, out_dtype, ld or 0)
@@ -1159,7 +1175,8 @@ def relpos_bias_1d(table, Nq, Nk, max_distance=128, bidirectional=True, q_offset
 def relpos_bias_1d_backward(dbias, num_buckets, max_distance=128, bidirectional=True, q_offset=0):
     """Gradient of relpos_bias_1d's table, f32 [num_buckets, H]: dbias [H, Nq, Nk] or [B, H, Nq, Nk] (the bias is shared by the batch; f32, fp16
     or bf16, any strides but the last) summed over the batch and over the pairs of each bucket."""
-    return _train("relpos_bias_1d_backward", dbias, _relpos_borders(int(num_buckets), int(max_distance), bool(bidirectional)), bool(bidirectional), q_offset)
+    borders = _borders(int(num_buckets), int(max_distance), bool(bidirectional))
+    return _train("relpos_bias_1d_backward", dbias, borders, bool(bidirectional), q_offset)
 
 
 def swin_relpos_bias_backward(dbias, ws):

@@ -77,6 +77,9 @@ relpos_fwd_kernel(const float* __restrict__ table, T* __restrict__ out, Borders 
   }
 }
 
+// Times below are of calls on one input again and again; the 134 MB of 8 x 8 x 1023^2 bf16 then stay in the last-level cache, where a call takes 35 us.
+// From memory, on inputs that take turns, it takes 46 us.
+//
 // Rows of a lane that are fetched at once: eight (8 x 8 x 1023^2 bf16 37 us, by fours 40 us); four where rows are so short that most of eight
 // would lie outside (9 x 20 x 3834 x 32 f32 34 us, by eights 42 us).
 constexpr int rows_in_flight(int lanes) { return lanes == 8 ? 4 : 8; }

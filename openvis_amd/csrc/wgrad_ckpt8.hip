@@ -12,10 +12,11 @@
 //   dY fp16: fp16 products; X is scaled per 32 columns by the largest scale of the workgroup's rows so that its largest code comes to at most
 //   57344: exact for scales down to 2^-22 of the largest.  A workgroup that meets a smaller one (rows far apart in size, the large ones perhaps
 //   with no gradient at all) throws its sums away and takes its rows again with dY as the sum of two bf16 numbers (11 bits: exact), which
-//   takes five times as long.  Blocks of the format's smallest scale, 2^-100, do not count: they are the zeros of padding and of ReLU; what
+//   takes about four times as long.  Blocks of the format's smallest scale, 2^-100, do not count: they are the zeros of padding and of ReLU; what
 //   values they hold, below 2^-91, are taken as 0 where the 32 columns' largest scale is 2^-77 or more.
 // All products are exact in f32; sums are f32.  Rows are split over workgroups (S parts) where there are too few tiles to fill the card; the
-// parts are added in a fixed order by a second kernel.  36928 x 1024 x 4096 fp16: 270 us, 1.15 PFLOP/s (2000 x 1000 x 1000: 27 us).
+// parts are added in a fixed order by a second kernel.  36928 x 1024 x 4096 fp16: 270 to 284 us by the card, 1.09 to
+// 1.15 PFLOP/s (2000 x 1000 x 1000: 24 us).
 #include "train_elem.h"
 #include <type_traits>
 
@@ -517,12 +518,16 @@ wgrad_join_kernel(const float* __restrict__ part, int S, const float* __restrict
 }
 
 struct WgradShape { int tile, tiles_n, tiles_k, S; long long chunk; int turns; };
-// Tile and split by a model of the time (us), fitted to sweeps over shapes of 100 to 294400 rows and 8 to 4096 columns:
+// Tile and split by a model of the time (us):
 //   a step of 32 rows takes `one` where a CU has one workgroup, and `more` longer for each further one, up to `most` at once; then they go in
 //   rounds.  16-bit: tile 256 1.0; 128 0.45 and 0.23; 64 0.43 and 0.22.  f32 (three products): 128 0.98 and 0.58; 64 0.45 and 0.25;
 //   S > 1 parts are written and read again at 4.5 TB/s, in a launch of its own.
-// 36928 x 1024 x 4096 fp16: tile 256 in 4 parts 328 us, 128 in 2 parts 405 us; 43120 x 512 x 512: 128 in 32 parts 55 us, 256 in 64 parts 67 us;
-// 500 x 2048 x 2048: 128 whole 21 us, 64 whole 31 us, 128 in 2 parts 33 us.
+// The constants were fitted to sweeps over shapes of 100 to 294400 rows and 8 to 4096 columns with an earlier form of the loop (tile 256's step takes
+// 0.88 us now).  What they choose is still the fastest of the tiles at each of these, us with tile 256 / 128 / 64, each in its own best split:
+//   fp16  36928 x 1024 x 4096 284 / 374 / 1243, 98500 x 768 x 768 134 / 157 / 488, 294400 x 192 x 768 146 / 164 / 374, 73600 x 384 x 1536 125 / 119 / 368,
+//         43120 x 512 x 512 63 / 52 / 110, 8192 x 1024 x 1024 47 / 40 / 86, 2000 x 1000 x 1000 34 / 24 / 33, 500 x 2048 x 2048 31 / 17 / 26,
+//         100 x 256 x 2048 21 / 10 / 8
+//   f32   36928 x 1024 x 4096 - / 900 / 1400, 43120 x 512 x 512 - / 86 / 110, 500 x 2048 x 2048 - / 25 / 27, 100 x 256 x 2048 - / 10 / 7
 inline WgradShape wgrad_shape(long long M, int N, int K, int dtype) {
   WgradShape best{};
   double least = 1e300;

@@ -1115,7 +1115,7 @@ def act_backward_ckpt8(dy, h8, act, recompute=False):
 def linear_wgrad_ckpt8(dy, x8, gamma=None, beta=None):
     """Gradients of a linear layer's weight [N, K] and bias [N] (f32): dy [..., N] and the layer's input as a Ckpt8 [rows, K] -> (dw, db).  With a
     layer norm's gamma / beta [K], x8 is its xhat8 and the layer's input was xhat * gamma + beta.  Every product is exact and the sums are f32; an
-    fp16 dy beside rows whose scales in one block of columns are more than 2^22 apart takes five times as long, and values below 2^-91 in blocks of
+    fp16 dy beside rows whose scales in one block of columns are more than 2^22 apart takes about four times as long, and values below 2^-91 in blocks of
     the smallest scale then count as 0."""
     return _train("linear_wgrad_ckpt8", dy, x8[0], x8[1], gamma, beta)
 
